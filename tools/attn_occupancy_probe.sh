@@ -11,7 +11,7 @@ build)
 	make -C "$CSRC" -j4 >/dev/null
 	mkdir -p "$OUT"
 	for kb in 16 48 112; do
-		/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I"$CSRC" -Wall -Wno-unused-function -ffp-contract=fast -DDEC_ATTN_DIAG_EXTRA_LDS=$((kb * 1024)) \
+		/opt/rocm/bin/hipcc -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I"$CSRC" -Wall -Wno-unused-function -ffp-contract=fast -DDEC_ATTN_DIAG_EXTRA_LDS=$((kb * 1024)) \
 			-c "$CSRC/attention.hip" -o "$OUT/attention_lds$kb.o"
 		objs=$(ls "$CSRC"/build/*.o | grep -v attention.hip.o)
 		/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o "$OUT/libnovic_hip_attnlds$kb.so" $objs "$OUT/attention_lds$kb.o"

@@ -50,7 +50,7 @@ DMA = re.compile(r"^\s*buffer_load_dword\w*\s.*\blds\b")
 
 def compile_asm(path):
 	out = tempfile.NamedTemporaryFile(suffix=".s", delete=False).name
-	cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-ffp-contract=fast", "-S",
+	cmd = ["/opt/rocm/bin/hipcc", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-O3", "-std=c++17", "--offload-arch=gfx950", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-ffp-contract=fast", "-S",
 	       "--cuda-device-only", path, "-o", out]
 	subprocess.run(cmd, check=True, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
 	with open(out) as f:

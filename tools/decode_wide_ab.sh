@@ -7,7 +7,7 @@ ROOT=$(cd "$(dirname "$0")/.." && pwd); CSRC=$ROOT/novic_amd/csrc; OUT=$ROOT/nov
 case "$1" in
 build)
 	make -C "$CSRC" -j4 >/dev/null; mkdir -p "$OUT"
-	/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I"$CSRC" -Wall -Wno-unused-function -ffp-contract=fast -DDECODE_LN_WIDE=0 -c "$CSRC/decode_fused.hip" -o "$OUT/decode_fused_narrow.o"
+	/opt/rocm/bin/hipcc -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I"$CSRC" -Wall -Wno-unused-function -ffp-contract=fast -DDECODE_LN_WIDE=0 -c "$CSRC/decode_fused.hip" -o "$OUT/decode_fused_narrow.o"
 	/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o "$OUT/libnovic_hip_lnnarrow.so" $(ls "$CSRC"/build/*.o | grep -v decode_fused.hip.o) "$OUT/decode_fused_narrow.o"
 	echo "built $OUT/libnovic_hip_lnnarrow.so";;
 run)

@@ -18,14 +18,14 @@ build|build-test)  # build-test: only the two libraries tests/test_gpu_schedule_
 		fi
 	fi
 	for d in $([ "$1" = build-test ] && echo 1 || echo 1 2 3); do
-		/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I"$CSRC" -Wall -Wno-unused-function -ffp-contract=fast -DWGRAD_DIAG=$d \
+		/opt/rocm/bin/hipcc -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I"$CSRC" -Wall -Wno-unused-function -ffp-contract=fast -DWGRAD_DIAG=$d \
 			-c "$CSRC/wgrad.hip" -o "$OUT/wgrad_d$d.o"
 		objs=$(ls "$CSRC"/build/*.o | grep -v wgrad.hip.o)
 		/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o "$OUT/libnovic_hip_wgdiag$d.so" $objs "$OUT/wgrad_d$d.o"
 		echo "built $OUT/libnovic_hip_wgdiag$d.so"
 	done
 	# the forward / input-gradient GEMM's four-phase K loop under the same per-wave delays (gemm256.hip, GEMM256_DIAG_JITTER)
-	/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I"$CSRC" -Wall -Wno-unused-function -ffp-contract=fast -DGEMM256_DIAG_JITTER=1 \
+	/opt/rocm/bin/hipcc -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I"$CSRC" -Wall -Wno-unused-function -ffp-contract=fast -DGEMM256_DIAG_JITTER=1 \
 		-c "$CSRC/gemm256.hip" -o "$OUT/gemm256_jit.o"
 	objs=$(ls "$CSRC"/build/*.o | grep -v gemm256.hip.o)
 	/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o "$OUT/libnovic_hip_g256jit.so" $objs "$OUT/gemm256_jit.o"
