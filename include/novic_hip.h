@@ -507,6 +507,57 @@ int novic_cache_gather_group(const float* embeds, const int* target_ids, const v
                              const int64_t* starts, int groups, int B_each, int64_t N, int F, int M_file, int C_file, int M, int C, float* out_embed, void* out_target,
                              uint8_t* out_mask, float* out_weight, int weight_mode, int64_t staged_row0, hipStream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Operators of decoder fine-tuning (no counterpart in the reference: it trains with cross entropy only).  Matrices of these calls have one of three element types and
+ * any row stride >= the row's width; a row may have any width and begin at any address its elements may have (no 16-byte alignment).  The main output may BE an input
+ * matrix of its own type and stride where a call's comment says so; any other overlap of an output is refused.  Workspaces are device memory of the size that the *_ws call names, 16-byte aligned, of any content,
+ * free again when the call's work on the stream is done.  Every sum is taken in a fixed order: the same inputs give the same bits.
+ * ------------------------------------------------------------------------------------------------------------ */
+enum { NOVIC_TYPE_F32 = 0, NOVIC_TYPE_BF16 = 1, NOVIC_TYPE_F16 = 2 };
+
+/* LayerNorm that keeps its row statistics: y[rows][E] = (x - mean) rstd gamma (+ beta), rstd = (var + eps)^-1/2; mean / rstd [rows] may be NULL.  y has x's type, or any type
+ * where x is fp32; gamma, beta [E] fp32; 1 <= E <= 16384.  y may be x.
+ * Backward: g = dy gamma, xhat = (x - mean) rstd; dx (x's type) = dx_in (NULL: 0) + rstd (g - mean_E(g) - xhat mean_E(g xhat)); dgamma / dbeta (either may be NULL)
+ * = sum_rows dy xhat / sum_rows dy, added to what they hold where accumulate is set.  dx may be dx_in, x or dy. */
+int novic_layernorm_stats_fwd(const void* x, int x_type, int64_t ldx, const float* gamma, const float* beta, void* y, int y_type, int64_t ldy, float* mean, float* rstd,
+                              int rows, int E, float eps, hipStream_t stream);
+uint64_t novic_layernorm_stats_bwd_ws(int rows, int E, int x_type, int y_type);
+int novic_layernorm_stats_bwd(const void* dy, int y_type, int64_t lddy, const void* x, int x_type, int64_t ldx, const float* gamma, const float* mean, const float* rstd,
+                              const void* dx_in, int64_t ldi, void* dx, int64_t lddx, float* dgamma, float* dbeta, int accumulate, int rows, int E, void* ws, uint64_t ws_bytes,
+                              hipStream_t stream);
+
+/* Dropout with a mask that is never stored: y[rows][cols] = (keep ? x * 65536 / (65536 - thr) : 0) (+ resid, of y's type), thr = round(65536 p).  Element i = row * cols + col is
+ * kept iff its 16 bits of Philox4x32-10 (key: seed; counter: i / 8 low, high, site, *step -- 0 where step is NULL; half i % 8 of the four words, low half first) are >= thr.
+ * The backward pass is the same call on dy without resid.  x and y have one type, or one of them is fp32.  y may be x or resid. */
+int novic_dropout(const void* x, int x_type, int64_t ldx, const void* resid, int64_t ldr, void* y, int y_type, int64_t ldy, int64_t rows, int64_t cols, double p, uint64_t seed,
+                  uint32_t site, const int64_t* step, hipStream_t stream);
+
+/* Token rows of the losses: logits [A T][ldl >= V], 1 <= V <= 2^28, target [A][ldt] token ids, pad [A][ldp] (may be NULL; 1 = padded).  Row a T + t counts if it is not padded and its target lies
+ * in [0, V); other rows' logits are not read, their outputs are zeros.  Columns V .. of dlogits are left as they are.  dlogits may be logits.
+ * logp [A][ldo] = x_target - logsumexp(x); lse [A T] (may be NULL).  Backward: dlogits = grad(a, t) ([v = target] - exp(x - lse)), grad(a, t) = grad[a grad_lda + t grad_ldt]. */
+int novic_token_logprobs(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int A, int T, int V,
+                         float* logp, int64_t ldo, float* lse, hipStream_t stream);
+int novic_token_logprobs_bwd(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int A, int T, int V,
+                             const float* lse, const float* grad, int64_t grad_lda, int64_t grad_ldt, void* dlogits, int64_t ldd, hipStream_t stream);
+
+/* Preference loss of n pairs: sequence i of the 2 n is preferred to sequence n + i.  z_i = beta (sum_t (logp - ref) of i - the same of n + i) over counted rows;
+ * loss = sum_i w_i l(z_i) / sum_i w_i (weight NULL: ones; no weight at all: loss and gradient are 0), l = -(1 - smoothing) log sigmoid(z) - smoothing log sigmoid(-z) |
+ * max(0, 1 - z) | ((z - 1/2) / beta)^2.  stats [3] = loss, weighted mean of z, sum of the weights; margin [n] = z, logp, dlogits = grad_scale dloss/dlogits may each be NULL. */
+enum { NOVIC_PREF_SIGMOID = 0, NOVIC_PREF_HINGE = 1, NOVIC_PREF_SQUARE = 2 };
+uint64_t novic_preference_loss_ws(int n, int T);
+int novic_preference_loss(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int n, int T, int V,
+                          const float* ref, int64_t ldref, const float* weight, int kind, double beta, double smoothing, double grad_scale, float* logp, int64_t ldo, float* margin,
+                          void* dlogits, int64_t ldd, float* stats, void* ws, uint64_t ws_bytes, hipStream_t stream);
+
+/* Clipped policy loss: q = exp(logp - old), a = adv[a adv_lda + t adv_ldt]: -min(q a, clip(q, 1 - clip_lo, 1 + clip_hi) a) + kl_coef (exp(ref - logp) - (ref - logp) - 1) (ref NULL:
+ * no such term), averaged over the counted rows, or (per_sequence) over the sequences that have any of the average over each one's counted rows; no counted row: all zeros.
+ * stats [4] = loss, KL, share of clipped rows (averaged the same way), counted rows; logp, dlogits = grad_scale dloss/dlogits may be NULL. */
+uint64_t novic_policy_loss_ws(int A, int T);
+int novic_policy_loss(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int A, int T, int V,
+                      const float* old_logp, int64_t ldold, const float* adv, int64_t adv_lda, int64_t adv_ldt, const float* ref, int64_t ldref, float clip_lo, float clip_hi,
+                      float kl_coef, int per_sequence, float grad_scale, float* logp, int64_t ldo, void* dlogits, int64_t ldd, float* stats, void* ws, uint64_t ws_bytes,
+                      hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -913,3 +913,262 @@ def beam_step_policy(generic: int = -1) -> int:
 def skinny_wide_policy(wide: int = -1) -> int:
 	"""0: four 128-column blocks (default), 1: two 256-column blocks for the [M x 512 x 512] bf16-store GEMM of the streaming kernel; returns the previous setting."""
 	return int(_lib.lib().novic_skinny_wide_policy(int(wide)))
+
+
+# ---- operators of decoder fine-tuning (csrc/layernorm_stats.hip, dropout.hip, token_loss.hip) ------------------------------------------------------------------------
+# Matrices are 2-D fp32 / bf16 / fp16 tensors with unit column stride, any row stride >= the width, any width and any (element-aligned) address.  Arguments are checked before
+# anything is launched: CPU tensors raise NovicHipError, wrong types TypeError, wrong shapes, strides and devices ValueError, an output that overlaps another tensor of the call
+# NovicHipError (the C ABI looks at the addresses; a main output may BE an input where a docstring says so).  The work is enqueued on the current stream of the tensors' device
+# (which need not be the current device); outputs are the caller's, a workspace is taken from torch's allocator for the one call, so that calls on several streams, and
+# captured graphs, never share one.  Nothing here records autograd history: a forward call has a backward call beside it.
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # NOVIC_TYPE_*
+PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "square": 2}       # NOVIC_PREF_*
+
+_C = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "u": ctypes.c_uint64, "w": ctypes.c_uint32, "f": ctypes.c_float, "d": ctypes.c_double}
+_SIGNATURES = {  # argument types in order; the stream comes last
+	"novic_layernorm_stats_fwd": "pilpppilppiifp",
+	"novic_layernorm_stats_bwd": "pilpilppp" + "plpl" + "ppiiipup",
+	"novic_dropout": "pilplpilll" + "duwpp",
+	"novic_token_logprobs": "pilpilpliii" + "plpp",
+	"novic_token_logprobs_bwd": "pilpilpliii" + "ppllplp",
+	"novic_preference_loss": "pilpilpliii" + "plpidddplpplppup",
+	"novic_policy_loss": "pilpilpliii" + "plpllplfffifplplppup",
+}
+_entries: dict = {}
+
+
+def _entry(name: str):
+	fn = _entries.get(name)
+	if fn is None:
+		fn = getattr(_lib.lib(), name)
+		fn.argtypes = [_C[c] for c in _SIGNATURES[name]]
+		_entries[name] = fn
+	return fn
+
+
+def _enqueue(name: str, device: torch.device, *args):
+	"""One C-ABI call on the current stream of `device`, with that device current while it is made."""
+	idx = device.index
+	if idx == torch._C._cuda_getDevice():
+		rc = _entry(name)(*args, torch._C._cuda_getCurrentRawStream(idx))
+	else:
+		with torch.cuda.device(idx):
+			rc = _entry(name)(*args, torch._C._cuda_getCurrentRawStream(idx))
+	if rc:
+		check(rc, name)
+
+
+def _bad_tensor(t, what: str, dtypes):
+	if not isinstance(t, torch.Tensor):
+		raise TypeError(f"{what}: a tensor, got {type(t).__name__}")
+	if not t.is_cuda:
+		raise _lib.NovicHipError("novic_amd kernels need tensors on an MI355X device (no CPU fallback exists)")
+	if t.dtype not in dtypes:
+		raise TypeError(f"{what}: {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
+
+
+def _matrix(t, what: str, device, rows, cols, dtypes=_TYPE):
+	"""(address, row stride) of a rows x cols matrix on `device` (None: any)."""
+	try:
+		r, c = t.shape
+		s, s1 = t.stride()
+		if t.dtype in dtypes and t.is_cuda and (rows is None or r == rows) and (cols is None or c == cols) and (device is None or t.device == device) and (s1 == 1 or c <= 1) and (s >= c or r <= 1):
+			return t.data_ptr(), s
+	except (AttributeError, ValueError):
+		pass
+	_bad_tensor(t, what, dtypes)
+	if device is not None and t.device != device:
+		raise ValueError(f"{what} is on {t.device}, not on {device}")
+	if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+		raise ValueError(f"{what}: a matrix of {'any' if rows is None else rows} x {'any' if cols is None else cols}, got {tuple(t.shape)}")
+	raise ValueError(f"{what}: unit column stride and a row stride of at least the width, got strides {t.stride()} for {tuple(t.shape)}")
+
+
+def _vector(t, what: str, device, n: int, dtype=torch.float32) -> int:
+	"""Address of n contiguous elements on `device`; 0 for None."""
+	if t is None:
+		return 0
+	try:
+		if t.dtype == dtype and t.device == device and t.numel() == n and t.is_contiguous():
+			return t.data_ptr()
+	except AttributeError:
+		pass
+	_bad_tensor(t, what, (dtype,))
+	raise ValueError(f"{what}: {n} contiguous elements on {device}, got {tuple(t.shape)} on {t.device}")
+
+
+def _given(t, what: str):
+	if t is None:
+		raise TypeError(f"{what}: a tensor, got None")
+	return t
+
+
+def layernorm_stats_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: Optional[torch.Tensor], out: torch.Tensor, mean: Optional[torch.Tensor] = None,
+                        rstd: Optional[torch.Tensor] = None, *, eps: float = 1e-5):
+	"""out = LayerNorm(x; gamma, beta) of a matrix [rows][E <= 16384] of any of the three types (out: x's type, or any type where x is fp32), keeping the rows' mean and rstd (fp32
+	[rows]) for layernorm_stats_bwd (novic_layernorm_stats_fwd).  gamma / beta: fp32 [E].  Beside layernorm_fwd, whose fp32 / fp16 rows of at most 2048 columns, a multiple of
+	4, need no statistics kept: its backward forms them again."""
+	px, ldx = _matrix(x, "x", None, None, None)
+	rows, E = x.shape
+	dev, xt = x.device, x.dtype
+	po, ldo = _matrix(out, "out", dev, rows, E, _TYPE if xt is torch.float32 else (xt,))
+	if not 1 <= E <= 16384:
+		raise ValueError(f"layernorm_stats_fwd: 1 <= width <= 16384, got {E}")
+	_enqueue("novic_layernorm_stats_fwd", dev, px, _TYPE[xt], ldx, _vector(_given(gamma, "gamma"), "gamma", dev, E), _vector(beta, "beta", dev, E), po, _TYPE[out.dtype], ldo,
+	         _vector(mean, "mean", dev, rows), _vector(rstd, "rstd", dev, rows), rows, E, eps)
+	return out
+
+
+def layernorm_stats_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, dx: torch.Tensor, dgamma: Optional[torch.Tensor] = None,
+                        dbeta: Optional[torch.Tensor] = None, *, dx_in: Optional[torch.Tensor] = None, accumulate: bool = False):
+	"""Backward of layernorm_stats_fwd (novic_layernorm_stats_bwd): dx (x's type) = dx_in (the residual branch's gradient, or None) + LayerNorm'(dy); dgamma / dbeta (fp32 [E], either
+	may be None) = the sums over the rows, added to what they hold with accumulate.  The sums have a fixed order: no atomics, the same bits every time.  dx may be dx_in, x or dy."""
+	px, ldx = _matrix(x, "x", None, None, None)
+	rows, E = x.shape
+	dev, xt = x.device, x.dtype
+	pdy, lddy = _matrix(dy, "dy", dev, rows, E, _TYPE if xt is torch.float32 else (xt,))
+	pdx, lddx = _matrix(dx, "dx", dev, rows, E, (xt,))
+	pin, ldi = _matrix(dx_in, "dx_in", dev, rows, E, (xt,)) if dx_in is not None else (0, 0)
+	if not 1 <= E <= 16384:
+		raise ValueError(f"layernorm_stats_bwd: 1 <= width <= 16384, got {E}")
+	pdg, pdb = _vector(dgamma, "dgamma", dev, E), _vector(dbeta, "dbeta", dev, E)
+	xi, yi = _TYPE[xt], _TYPE[dy.dtype]
+	need = _ws_bytes("novic_layernorm_stats_bwd_ws", rows, E, xi, yi) if pdg or pdb else 0
+	ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+	_enqueue("novic_layernorm_stats_bwd", dev, pdy, yi, lddy, px, xi, ldx, _vector(_given(gamma, "gamma"), "gamma", dev, E), _vector(_given(mean, "mean"), "mean", dev, rows),
+	         _vector(_given(rstd, "rstd"), "rstd", dev, rows), pin, ldi, pdx, lddx, pdg, pdb, int(accumulate), rows, E, 0 if ws is None else ws.data_ptr(), need)
+	return dx
+
+
+def _dropout(x, out, dropout, resid, step):
+	px, ldx = _matrix(x, "input", None, None, None)
+	rows, cols = x.shape
+	dev, xt, yt = x.device, x.dtype, getattr(out, "dtype", None)
+	po, ldo = _matrix(out, "out", dev, rows, cols, _TYPE if xt is torch.float32 else (xt, torch.float32))
+	if not 0.0 <= dropout.p <= 1.0:
+		raise ValueError(f"dropout probability in [0, 1], got {dropout.p}")
+	pr, ldr = _matrix(resid, "resid", dev, rows, cols, (yt,)) if resid is not None else (0, 0)
+	_enqueue("novic_dropout", dev, px, _TYPE[xt], ldx, pr, ldr, po, _TYPE[yt], ldo, rows, cols, dropout.p, dropout.seed & 0xFFFFFFFFFFFFFFFF, dropout.site & 0xFFFFFFFF,
+	         _vector(step, "step", dev, 1, torch.int64))
+	return out
+
+
+def dropout_fwd(x: torch.Tensor, out: torch.Tensor, dropout: Dropout, *, resid: Optional[torch.Tensor] = None, step: Optional[torch.Tensor] = None):
+	"""out = dropout(x) (+ resid, of out's type) of a matrix [rows][cols] (novic_dropout).  The mask is Philox4x32-10 of (dropout.seed, dropout.site, *step, element index) with 16
+	bits an element: never stored, drawn again by dropout_bwd with the same descriptor and step.  step: an int64 device scalar that a captured graph can count up, so that each
+	replay drops other elements (None: 0).  Kept elements are scaled by 65536 / (65536 - round(65536 p)); dropped ones are zeros, whatever they were.  p = 1 drops all.
+	NOT the masks of the dropout that gemm() and the fused decoder kernels carry in their epilogues (csrc/common.hpp: an avalanche hash of the same triple)."""
+	return _dropout(x, out, dropout, resid, step)
+
+
+def dropout_bwd(dy: torch.Tensor, dx: torch.Tensor, dropout: Dropout, *, step: Optional[torch.Tensor] = None):
+	"""dx = the gradient of dropout_fwd's input: dy under the same mask and scale (the residual's gradient is dy itself)."""
+	return _dropout(dy, dx, dropout, None, step)
+
+
+_TOKENS = (torch.int64, torch.int32)
+_MASKS = (torch.bool, torch.uint8)
+_F32 = (torch.float32,)
+
+
+def _token_rows(logits, target, pad):
+	"""Checks what the token operators share; (device, A, T, V, the C ABI's leading arguments)."""
+	pl, ldl = _matrix(logits, "logits", None, None, None)
+	dev = logits.device
+	pt, ldt = _matrix(target, "target", dev, None, None, _TOKENS)
+	A, T = target.shape
+	R, V = logits.shape
+	if R != A * T:
+		raise ValueError(f"logits: one row for each of the {A} x {T} target positions, got {R}")
+	if V < 1 or R >= 1 << 31:
+		raise ValueError("token rows: a vocabulary of at least one, at most 2^31 - 1 rows")
+	pp, ldp = _matrix(pad, "pad", dev, A, T, _MASKS) if pad is not None else (0, 0)
+	return dev, A, T, V, (pl, _TYPE[logits.dtype], ldl, pt, target.element_size(), ldt, pp, ldp)
+
+
+def _optional(t, what, dev, rows, cols, dtypes):
+	return _matrix(t, what, dev, rows, cols, dtypes) if t is not None else (0, 0)
+
+
+def _per_token(t, what, dev, A, T):
+	"""(address, strides) of an fp32 [A][T] tensor, or of [A] as one value a sequence."""
+	if isinstance(t, torch.Tensor) and t.dim() == 1:
+		return _vector(t, what, dev, A), 1, 0
+	return (*_matrix(t, what, dev, A, T, _F32), 1)
+
+
+def _ws_bytes(name: str, *sizes) -> int:
+	ask = _entries.get(name)
+	if ask is None:
+		ask = getattr(_lib.lib(), name)
+		ask.restype, ask.argtypes = ctypes.c_uint64, [ctypes.c_int] * len(sizes)
+		_entries[name] = ask
+	return ask(*sizes)
+
+
+def token_logprobs(logits: torch.Tensor, target: torch.Tensor, out: torch.Tensor, *, pad: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
+	"""out [A][T] (fp32) = log softmax(logits row a T + t)[target[a][t]] (novic_token_logprobs): what the losses below take as `ref` / `old` from a frozen decoder.  logits
+	[A T][V] of any of the three types (a column window of a wider buffer keeps its row stride), target [A][T] int64 / int32, pad [A][T] bool (True: padded).  Positions that are
+	padded or whose target lies outside [0, V) do not count: 0, and their logits are not read.  lse [A T] (fp32): the rows' log-sum-exp for token_logprobs_bwd."""
+	dev, A, T, V, head = _token_rows(logits, target, pad)
+	po, ldo = _matrix(out, "out", dev, A, T, _F32)
+	_enqueue("novic_token_logprobs", dev, *head, A, T, V, po, ldo, _vector(lse, "lse", dev, A * T))
+	return out
+
+
+def token_logprobs_bwd(logits: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor, dlogits: torch.Tensor, *, pad: Optional[torch.Tensor] = None):
+	"""dlogits (logits' type, may be logits) = grad[a][t] ([v = target] - exp(logits - lse)); zeros where a position does not count (novic_token_logprobs_bwd).  grad: fp32 [A][T], or
+	[A] for a gradient that all positions of a sequence share (the backward of a sequence's sum)."""
+	dev, A, T, V, head = _token_rows(logits, target, pad)
+	pd, ldd = _matrix(dlogits, "dlogits", dev, A * T, V, (logits.dtype,))
+	_enqueue("novic_token_logprobs_bwd", dev, *head, A, T, V, _vector(_given(lse, "lse"), "lse", dev, A * T), *_per_token(grad, "grad", dev, A, T), pd, ldd)
+	return dlogits
+
+
+def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref: torch.Tensor, stats: torch.Tensor, *, beta: float, kind: str = "sigmoid", smoothing: float = 0.0,
+                    pad: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None, logp: Optional[torch.Tensor] = None, margin: Optional[torch.Tensor] = None,
+                    dlogits: Optional[torch.Tensor] = None, grad_scale: float = 1.0):
+	"""Loss of n preferences and its gradient (novic_preference_loss).  The first n of the A = 2 n sequences are each preferred to the one n behind it: z = beta (sum over the counted
+	positions of logp - ref, of the one minus of the other), ref [A][T] (fp32) the token log-probabilities under the frozen decoder (token_logprobs).
+	kind: "sigmoid" -(1 - smoothing) log sigmoid(z) - smoothing log sigmoid(-z), "hinge" max(0, 1 - z), "square" ((z - 1/2) / beta)^2; averaged with weight (fp32 [n], None: ones).
+	stats (fp32 [3]) = loss, mean margin, sum of the weights; margin (fp32 [n]) = z; logp (fp32 [A][T]); dlogits (logits' type, may be logits) = grad_scale * gradient, zeros where a
+	position does not count.  Rows, targets and pad as in token_logprobs.  As cross_entropy, one call makes the loss and the gradient: grad_scale is the upstream gradient."""
+	dev, A, T, V, head = _token_rows(logits, target, pad)
+	if A < 2 or A % 2 or T < 1:
+		raise ValueError(f"preference_loss: an even number of sequences, preferred ones first, of at least one position, got {A} x {T}")
+	n = A // 2
+	if kind not in PREFERENCE_KINDS:
+		raise ValueError(f"preference_loss: kind is one of {', '.join(PREFERENCE_KINDS)}, got {kind!r}")
+	if not beta > 0.0 or not 0.0 <= smoothing < 0.5 or (smoothing != 0.0 and kind != "sigmoid"):
+		raise ValueError("preference_loss: beta > 0, smoothing in [0, 0.5) and with the sigmoid form only")
+	pref, ldref = _matrix(ref, "ref", dev, A, T, _F32)
+	plp, ldo = _optional(logp, "logp", dev, A, T, _F32)
+	pd, ldd = _optional(dlogits, "dlogits", dev, A * T, V, (logits.dtype,))
+	ws = torch.empty(_ws_bytes("novic_preference_loss_ws", n, T), dtype=torch.uint8, device=dev)
+	_enqueue("novic_preference_loss", dev, *head, n, T, V, pref, ldref, _vector(weight, "weight", dev, n), PREFERENCE_KINDS[kind], beta, smoothing, grad_scale, plp, ldo,
+	         _vector(margin, "margin", dev, n), pd, ldd, _vector(_given(stats, "stats"), "stats", dev, 3), ws.data_ptr(), ws.numel())
+	return stats
+
+
+def policy_loss(logits: torch.Tensor, target: torch.Tensor, old: torch.Tensor, advantage: torch.Tensor, stats: torch.Tensor, *, clip=(0.2, 0.2), ref: Optional[torch.Tensor] = None,
+                kl_coef: float = 0.0, per_sequence: bool = False, pad: Optional[torch.Tensor] = None, logp: Optional[torch.Tensor] = None, dlogits: Optional[torch.Tensor] = None,
+                grad_scale: float = 1.0):
+	"""Clipped policy loss with a KL term and its gradient (novic_policy_loss).  target holds sampled tokens, old [A][T] (fp32) their log-probabilities when they were sampled,
+	advantage fp32 [A] or [A][T]: -min(q a, clip(q, 1 - clip[0], 1 + clip[1]) a) with q = exp(logp - old), plus kl_coef (exp(d) - d - 1), d = ref - logp, where ref [A][T] is given;
+	averaged over the counted positions, or (per_sequence) over each sequence's and then over the sequences that have any.  stats (fp32 [4]) = loss, KL, clipped share (averaged
+	alike), counted positions; all zeros, gradient too, where no position counts.  logp, dlogits, grad_scale as in preference_loss."""
+	dev, A, T, V, head = _token_rows(logits, target, pad)
+	if A < 1 or T < 1:
+		raise ValueError(f"policy_loss: at least one sequence of one position, got {A} x {T}")
+	lo, hi = clip
+	if not 0.0 <= lo <= 1.0 or not hi >= 0.0 or not kl_coef >= 0.0:
+		raise ValueError("policy_loss: 0 <= clip[0] <= 1, clip[1] >= 0, kl_coef >= 0")
+	pold, ldold = _matrix(old, "old", dev, A, T, _F32)
+	padv = _per_token(advantage, "advantage", dev, A, T)
+	pref, ldref = _optional(ref, "ref", dev, A, T, _F32)
+	plp, ldo = _optional(logp, "logp", dev, A, T, _F32)
+	pd, ldd = _optional(dlogits, "dlogits", dev, A * T, V, (logits.dtype,))
+	ws = torch.empty(_ws_bytes("novic_policy_loss_ws", A, T), dtype=torch.uint8, device=dev)
+	_enqueue("novic_policy_loss", dev, *head, A, T, V, pold, ldold, *padv, pref, ldref, lo, hi, kl_coef, int(per_sequence), grad_scale, plp, ldo, pd, ldd,
+	         _vector(_given(stats, "stats"), "stats", dev, 4), ws.data_ptr(), ws.numel())
+	return stats
