@@ -11,6 +11,9 @@
 #include "novic_hip.h"
 #include "rowvec.hpp"
 
+#ifndef DROP_NT
+#define DROP_NT false
+#endif
 namespace {
 
 struct Args {
@@ -58,7 +61,7 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(const Args g) {
 			if (RESID) t += r.get(i);
 			o[i] = t;
 		}
-		store_vec<YT, 8>(y + 8 * b, o);
+		store_vec<DROP_NT>(y + 8 * b, o);
 	}
 	if (first == 0 && (n & 7)) {  // the last, partial block
 		bool keep[8];
@@ -96,7 +99,7 @@ __global__ __launch_bounds__(256) void dropout_rows_kernel(const Args g) {
 					if (RESID) t += r.get(i);
 					o[i] = t;
 				}
-				store_vec<YT, 8>(y + e, o);
+				store_vec<DROP_NT>(y + e, o);
 			} else {
 #pragma unroll
 				for (int i = 0; i < 8; ++i) {

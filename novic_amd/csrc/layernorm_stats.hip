@@ -96,7 +96,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_fwd
 				if (beta) t += bt[c].get(i);
 				o[i] = t;
 			}
-			store_own<YT, CH>(y + (long long)row * ldy, es[c], (c * LANES + lane) * CH, o);
+			store_own<false>(y + (long long)row * ldy, es[c], (c * LANES + lane) * CH, o);
 		}
 	}
 }
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_bwd
 				if (dx_in) t += cur.in[c].get(i);
 				o[i] = t;
 			}
-			store_own<XT, CH>(dx + (long long)row * lddx, es[c], (c * LANES + lane) * CH, o);
+			store_own<true>(dx + (long long)row * lddx, es[c], (c * LANES + lane) * CH, o);
 		}
 		if (AHEAD) cur = nxt;
 	}
@@ -343,7 +343,9 @@ extern "C" int novic_layernorm_stats_bwd(const void* dy, int y_type, int64_t ldd
 	NOVIC_CHECK(!affine || rows == 0 || direct || (ws && ws_bytes >= (uint64_t)p.blocks * E * 8), "novic_layernorm_stats_bwd: the workspace is smaller than novic_layernorm_stats_bwd_ws says");
 	float* pg = !dgamma ? nullptr : direct ? dgamma : (float*)ws;
 	float* pb = !dbeta ? nullptr : direct ? dbeta : (float*)ws + (size_t)p.blocks * E;
-	if (rows > 0) NOVIC_LN_TYPES(launch_bwd, p, dy, lddy, x, ldx, gamma, mean, rstd, dx_in, ldi, dx, lddx, pg, pb, rows, E, direct && accumulate, stream)
+	if (rows > 0) {
+		NOVIC_LN_TYPES(launch_bwd, p, dy, lddy, x, ldx, gamma, mean, rstd, dx_in, ldi, dx, lddx, pg, pb, rows, E, direct && accumulate, stream)
+	}
 	if (affine && (rows == 0 ? !accumulate : !direct))  // (no rows: the sums are zero)
 		layernorm_stats_reduce_kernel<<<dim3((E + 31) / 32, 2), dim3(1024), 0, stream>>>(pg, pb, dgamma, dbeta, rows == 0 ? 0 : p.blocks, E, accumulate);
 	NOVIC_LAUNCH_CHECK();

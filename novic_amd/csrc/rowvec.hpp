@@ -16,9 +16,7 @@ struct RawVec {
 		} else if constexpr (__is_same(T, bf16)) {
 			return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
 		} else {
-			T h[2];
-			__builtin_memcpy(h, &w[i / 2], 4);
-			return (float)h[i & 1];
+			return (float)__builtin_bit_cast(T, (unsigned short)(i & 1 ? w[i / 2] >> 16 : w[i / 2]));
 		}
 	}
 	__device__ __forceinline__ void put(const float (&f)[N]) {
@@ -56,11 +54,21 @@ template <typename T>
 __device__ __forceinline__ const T* elem(const T* row, int e) {
 	return (const T*)((const char*)row + (uint32_t)e * (uint32_t)sizeof(T));
 }
-template <typename T, int N>
+// STREAM: past the caches (an output larger than they are, which nobody finds there again, leaves them to the inputs)
+template <bool STREAM, typename T, int N>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
 	RawVec<T, N> r;
 	r.put(f);
-	__builtin_memcpy(p, &r, sizeof(r));
+	if constexpr (STREAM && sizeof(r) % 16 == 0) {
+		typedef uint32_t quad __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+		for (int i = 0; i < (int)sizeof(r) / 16; ++i) {
+			const quad q = {r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
+			__builtin_nontemporal_store(q, (quad*)p + i);
+		}
+	} else {
+		__builtin_memcpy(p, &r, sizeof(r));
+	}
 }
 // The same values, out of the compiler's sight: what is computed from them again is not kept in registers over the code between.
 template <typename T, int N>
@@ -71,10 +79,10 @@ __device__ __forceinline__ void forget(RawVec<T, N>& r) {
 	}
 }
 // the elements e0 .. of a chunk that was loaded at es <= e0, at row p
-template <typename T, int N>
+template <bool STREAM, typename T, int N>
 __device__ __forceinline__ void store_own(T* p, int es, int e0, const float (&f)[N]) {
 	if (es == e0) {
-		store_vec<T, N>(elem(p, es), f);
+		store_vec<STREAM>(elem(p, es), f);
 	} else {
 #pragma unroll
 		for (int i = 1; i < N; ++i)

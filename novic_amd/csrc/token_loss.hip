@@ -16,6 +16,11 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+// A row's sums are seen from M = fl(m log2 e), m its maximum: an exponential is one fma and one v_exp_f32, exp2(x LOG2E - M), and M's rounding takes part in nothing but the choice
+// of the point, m' = M / LOG2E, from which x - m' is measured (in fp64, once a row).
+__device__ __forceinline__ float expo(float x, float M) { return __builtin_amdgcn_exp2f(fmaf(x, LOG2E, -M)); }
+__device__ __forceinline__ float point(float m) { return m * LOG2E; }
+__device__ __forceinline__ double from_point(float M) { return (double)M / (double)LOG2E; }
 
 struct Rows {
 	const void* logits;
@@ -28,10 +33,10 @@ struct Rows {
 	int tok_bytes, A, T, V;
 };
 
-__device__ __forceinline__ int counted_target(const Rows& g, int a, int t) {  // -1: the position does not count
-	if (g.pad && g.pad[a * g.ldp + t]) return -1;
+__device__ __forceinline__ int counted_target(const Rows& g, int a, int t) {  // -1: the position does not count (mask and target are requested together)
+	const bool padded = g.pad && g.pad[a * g.ldp + t];
 	const long long v = g.tok_bytes == 8 ? ((const long long*)g.target)[a * g.ldt + t] : (long long)((const int*)g.target)[a * g.ldt + t];
-	return v < 0 || v >= g.V ? -1 : (int)v;
+	return padded || v < 0 || v >= g.V ? -1 : (int)v;
 }
 
 // Workgroup -> row.  A grid's extent in threads is 32 bits, so rows beyond 2^20 go to its second dimension.
@@ -80,7 +85,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 template <typename T, int CH, int THREADS, int NC>
 struct RowTile {
 	float x[NC][CH];
-	float m, s;
+	float M, s;
 	__device__ __forceinline__ static int own(int c) { return (c * THREADS + (int)threadIdx.x) * CH; }
 	__device__ __forceinline__ static int at(int c, int V) { return min(own(c), V - CH); }
 	__device__ __forceinline__ void load(const T* row, int V) {
@@ -99,7 +104,7 @@ struct RowTile {
 		for (int c = 0; c < NC; ++c)
 #pragma unroll
 			for (int i = 0; i < CH; ++i) t = fmaxf(t, x[c][i]);
-		m = block_max<THREADS>(t, red);
+		M = point(block_max<THREADS>(t, red));
 		t = 0.f;
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
@@ -110,53 +115,132 @@ struct RowTile {
 			}
 #pragma unroll
 			for (int i = 0; i < CH; ++i) {
-				x[c][i] = __builtin_amdgcn_exp2f((x[c][i] - m) * LOG2E);
+				x[c][i] = expo(x[c][i], M);
 				if ((c + 1) * THREADS * CH > V && at(c, V) + i < own(c)) x[c][i] = 0.f;
 				t += x[c][i];
 			}
 		}
 		s = block_sum<THREADS>(t, red + THREADS / 64);
 	}
-	// dlogits = g ([v = target] - x / s)
-	__device__ __forceinline__ void grad(T* row, int V, int target, float g) {
+	// dlogits = g ([v = target] - x / s); the target's element is stored once more by the lane that owns it, which costs less than a comparison an element
+	__device__ __forceinline__ void grad(T* row, int V, int target, float et, float g) {
 		const float k = -g / s;
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
 			if (own(c) >= V) continue;
 			float o[CH];
-			const int es = at(c, V);
 #pragma unroll
-			for (int i = 0; i < CH; ++i) o[i] = (k * x[c][i] + (es + i == target ? g : 0.f));
-			store_own<T, CH>(row, es, own(c), o);
+			for (int i = 0; i < CH; ++i) o[i] = k * x[c][i];
+			store_own<true>(row, at(c, V), own(c), o);
 		}
+		if ((target / CH) % THREADS == (int)threadIdx.x) row[target] = (T)(k * et + g);
 	}
 };
 
-template <typename T, int CH, int THREADS>
-__device__ __forceinline__ void zero_row(T* row, int V) {
-	float o[CH];
+// A row in passing, by a team of LANES lanes: UNROLL vectors a lane are requested at once.
+template <typename T, int CH, int LANES, int UNROLL = 4>
+struct RowStream {
+	// (vectors that all lanes have whole are addressed from a scalar base and the one offset of the lane)
+	__device__ __forceinline__ static void load(RawVec<T, CH> (&raw)[UNROLL], const T* row, int e, int V, int lane) {
+		if (e + UNROLL * LANES * CH <= V) {
 #pragma unroll
-	for (int i = 0; i < CH; ++i) o[i] = 0.f;
-	for (int e0 = threadIdx.x * CH; e0 < V; e0 += THREADS * CH) store_own<T, CH>(row, min(e0, V - CH), e0, o);
-}
+			for (int u = 0; u < UNROLL; ++u) raw[u] = load_vec<T, CH>(elem(row + (e + u * LANES * CH), lane * CH));
+		} else {
+#pragma unroll
+			for (int u = 0; u < UNROLL; ++u) raw[u] = load_vec<T, CH>(elem(row, min(e + (u * LANES + lane) * CH, V - CH)));
+		}
+	}
+	// point and sum over this lane's part, with a running maximum
+	__device__ __forceinline__ static void sum(const T* row, int V, int lane, float& tM, float& ts) {
+		tM = -INFINITY;
+		ts = 0.f;
+		for (int e = 0; e < V; e += UNROLL * LANES * CH) {
+			RawVec<T, CH> raw[UNROLL];
+			load(raw, row, e, V, lane);
+			float top = -INFINITY;
+#pragma unroll
+			for (int u = 0; u < UNROLL; ++u) {
+#pragma unroll
+				for (int i = 0; i < CH; ++i) top = fmaxf(top, raw[u].get(i));
+				forget(raw[u]);  // (else its elements stay unpacked from one use to the next, at twice the registers)
+			}
+			const float M = fmaxf(tM, point(top)), base = M == -INFINITY ? 0.f : M;  // (nothing but -inf yet: their exponentials are zeros)
+			ts *= __builtin_amdgcn_exp2f(tM - base);
+			if (e + UNROLL * LANES * CH <= V) {
+#pragma unroll
+				for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+					for (int i = 0; i < CH; ++i) ts += expo(raw[u].get(i), base);
+			} else {
+#pragma unroll
+				for (int u = 0; u < UNROLL; ++u) {
+					const int e0 = e + (u * LANES + lane) * CH, es = min(e0, V - CH);
+#pragma unroll
+					for (int i = 0; i < CH; ++i) ts += es + i >= e0 ? expo(raw[u].get(i), base) : 0.f;
+				}
+			}
+			tM = M;
+		}
+	}
+	// a lane's sum seen from the row's point
+	__device__ __forceinline__ static float scaled(float tM, float ts, float M) {
+		const float base = M == -INFINITY ? 0.f : M;
+		return ts * __builtin_amdgcn_exp2f((tM == -INFINITY ? base : tM) - base);
+	}
+	// out = k exp2(x log2 e - M), and coef more at the target (whose logit is xt); out may be row
+	__device__ __forceinline__ static void grad(const T* row, T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
+		for (int e = 0; e < V; e += UNROLL * LANES * CH) {
+			RawVec<T, CH> raw[UNROLL];
+			load(raw, row, e, V, lane);
+#pragma unroll
+			for (int u = 0; u < UNROLL; ++u) {
+				float o[CH];
+#pragma unroll
+				for (int i = 0; i < CH; ++i) o[i] = k * expo(raw[u].get(i), M);
+				if (e + UNROLL * LANES * CH <= V) {
+					store_vec<true>(elem(out + (e + u * LANES * CH), lane * CH), o);
+				} else {
+					const int e0 = e + (u * LANES + lane) * CH;
+					if (e0 < V) store_own<true>(out, min(e0, V - CH), e0, o);
+				}
+			}
+		}
+		if ((target / CH) % LANES == lane) out[target] = (T)(k * expo(xt, M) + coef);
+	}
+	__device__ __forceinline__ static void zero(T* row, int V, int lane) {
+		float o[CH];
+#pragma unroll
+		for (int i = 0; i < CH; ++i) o[i] = 0.f;
+		for (int e0 = lane * CH; e0 < V; e0 += LANES * CH) store_own<true>(row, min(e0, V - CH), e0, o);
+	}
+};
 
 // ---- log-probabilities -------------------------------------------------------------------------------------------------------------------------------------------
 struct LogpOut {
 	float* logp;       // [A][T] or null
-	float* lse;        // [A T] or null: m + log(s)
+	float* lse;        // [A T] or null: the row's log-sum-exp
 	const float* ref;  // [A][T] or null
 	double* diff;      // [A T] or null: lp - ref, 0 where the row does not count
-	float2* norm;      // [A T] or null: (m, 1 / s)
+	float2* norm;      // [A T] or null: (M, 1 / s)
 	long long ldo, ldref;
 };
-__device__ __forceinline__ void put_logp(const LogpOut& o, int r, int a, int t, bool counts, double lp, float m, float s) {
+__device__ __forceinline__ float reference(const LogpOut& o, int a, int t) { return o.diff ? o.ref[a * o.ldref + t] : 0.f; }
+__device__ __forceinline__ void put_logp(const LogpOut& o, int r, int a, int t, bool counts, double lp, float M, float s, float ref = 0.f) {
 	if (o.logp) o.logp[a * o.ldo + t] = counts ? (float)lp : 0.f;
-	if (o.lse) o.lse[r] = counts ? (float)((double)m + log_wide(s)) : 0.f;
-	if (o.diff) o.diff[r] = counts ? lp - (double)o.ref[a * o.ldref + t] : 0.0;
-	if (o.norm) o.norm[r] = counts ? make_float2(m, 1.f / s) : make_float2(0.f, 0.f);
+	if (o.lse) o.lse[r] = counts ? (float)(from_point(M) + log_wide(s)) : 0.f;
+	if (o.diff) o.diff[r] = counts ? lp - (double)ref : 0.0;
+	if (o.norm) o.norm[r] = counts ? make_float2(M, 1.f / s) : make_float2(0.f, 0.f);
 }
 
-template <typename T, int CH, int THREADS, int NC>
+template <typename T, int CH, int THREADS>
+__device__ __forceinline__ void block_row_sum(const T* row, int V, float* red, float& M, float& s) {
+	float tM, ts;
+	RowStream<T, CH, THREADS>::sum(row, V, threadIdx.x, tM, ts);
+	M = block_max<THREADS>(tM, red);
+	s = block_sum<THREADS>(RowStream<T, CH, THREADS>::scaled(tM, ts, M), red + THREADS / 64);
+}
+__device__ __forceinline__ double row_logp(float xt, float M, float s) { return ((double)xt - from_point(M)) - log_wide(s); }
+template <typename T, int CH, int THREADS>
 __global__ __launch_bounds__(THREADS) void logp_kernel(const Rows g, const LogpOut o) {
 	__shared__ float red[2 * THREADS / 64];
 	const int r = row_index(g);
@@ -168,55 +252,16 @@ __global__ __launch_bounds__(THREADS) void logp_kernel(const Rows g, const LogpO
 		return;
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
-	RowTile<T, CH, THREADS, NC> tile;
-	tile.load(row, g.V);
-	const float xt = (float)row[target];
-	tile.sum(g.V, red);
-	if (threadIdx.x == 0) put_logp(o, r, a, t, true, ((double)xt - (double)tile.m) - log_wide(tile.s), tile.m, tile.s);
-}
-
-// rows beyond the register forms: maximum and sum in one pass with a running maximum
-template <typename T, int CH, int THREADS>
-__device__ __forceinline__ void long_row_sum(const T* row, int V, float* red, float& m, float& s) {
-	float tm = -INFINITY, ts = 0.f;
-	for (int e0 = threadIdx.x * CH; e0 < V; e0 += THREADS * CH) {
-		const int es = min(e0, V - CH);
-		const RawVec<T, CH> raw = load_vec<T, CH>(elem(row, es));
-		float top = tm;
-#pragma unroll
-		for (int i = 0; i < CH; ++i) top = fmaxf(top, raw.get(i));
-		const float base = top == -INFINITY ? 0.f : top;  // (nothing but -inf yet: their exponentials are zeros)
-		ts *= __builtin_amdgcn_exp2f((tm - base) * LOG2E);
-#pragma unroll
-		for (int i = 0; i < CH; ++i) ts += es + i >= e0 ? __builtin_amdgcn_exp2f((raw.get(i) - base) * LOG2E) : 0.f;
-		tm = top;
-	}
-	m = block_max<THREADS>(tm, red);
-	const float base = m == -INFINITY ? 0.f : m;
-	s = block_sum<THREADS>(ts * __builtin_amdgcn_exp2f(((tm == -INFINITY ? base : tm) - base) * LOG2E), red + THREADS / 64);
-}
-template <typename T, int CH, int THREADS>
-__global__ __launch_bounds__(THREADS) void logp_long_kernel(const Rows g, const LogpOut o) {
-	__shared__ float red[2 * THREADS / 64];
-	const int r = row_index(g);
-	if (r < 0) return;
-	const int a = r / g.T, t = r - a * g.T;
-	const int target = counted_target(g, a, t);
-	if (target < 0) {
-		if (threadIdx.x == 0) put_logp(o, r, a, t, false, 0.0, 0.f, 1.f);
-		return;
-	}
-	const T* row = (const T*)g.logits + (long long)r * g.ldl;
-	const float xt = (float)row[target];
-	float m, s;
-	long_row_sum<T, CH, THREADS>(row, g.V, red, m, s);
-	if (threadIdx.x == 0) put_logp(o, r, a, t, true, ((double)xt - (double)m) - log_wide(s), m, s);
+	const float xt = (float)row[target], ref = reference(o, a, t);
+	float M, s;
+	block_row_sum<T, CH, THREADS>(row, g.V, red, M, s);
+	if (threadIdx.x == 0) put_logp(o, r, a, t, true, row_logp(xt, M, s), M, s, ref);
 }
 
 // ---- gradient of log-probabilities: dlogits = coef (1[v = target] - exp(x - m) / s) ----------------------------------------------------------------------------------
 struct GradIn {
-	const float* lse;     // [A T] (m + log s), or null:
-	const float2* norm;   // [A T] (m, 1 / s)
+	const float* lse;     // [A T], or null:
+	const float2* norm;   // [A T] (M, 1 / s)
 	const float* grad;    // element (a, t) at grad[a * lda + t * ldt]
 	long long lda, ldt;
 	const float* scale;   // device scalar or null
@@ -229,28 +274,24 @@ __global__ __launch_bounds__(THREADS) void logp_grad_kernel(const Rows g, const 
 	const int target = counted_target(g, a, t);
 	T* out = (T*)g.dlogits + (long long)r * g.ldd;
 	if (target < 0) {
-		zero_row<T, CH, THREADS>(out, g.V);
+		RowStream<T, CH, THREADS>::zero(out, g.V, threadIdx.x);
 		return;
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
 	float coef = in.grad[a * in.lda + t * in.ldt];
 	if (in.scale) coef *= *in.scale;
-	float m, k = -coef;
+	float M, k = -coef;
 	if (in.norm) {
 		const float2 n = in.norm[r];
-		m = n.x;
+		M = n.x;
 		k *= n.y;
 	} else {
-		m = in.lse[r];
+		const float lse = in.lse[r];
+		M = point(lse);
+		k *= __builtin_amdgcn_exp2f(-fmaf(lse, LOG2E, -M));  // (what the point's rounding took: s is what lse says, seen from M)
 	}
-	for (int e0 = threadIdx.x * CH; e0 < g.V; e0 += THREADS * CH) {
-		const int es = min(e0, g.V - CH);
-		const RawVec<T, CH> raw = load_vec<T, CH>(elem(row, es));
-		float o[CH];
-#pragma unroll
-		for (int i = 0; i < CH; ++i) o[i] = (k * __builtin_amdgcn_exp2f((raw.get(i) - m) * LOG2E) + (es + i == target ? coef : 0.f));
-		store_own<T, CH>(out, es, e0, o);
-	}
+	const float xt = (float)row[target];  // (used by the lane that owns the target alone, which loads it before it writes there: out may be row)
+	RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, M, k, coef);
 }
 
 // ---- preference loss ---------------------------------------------------------------------------------------------------------------------------------------------
@@ -260,47 +301,56 @@ struct Pref {
 	int n, T, kind;
 	double beta, smoothing, grad_scale;
 	float* margin;        // [n] or null
-	float* coef;          // [2 n]: gradient of the loss to a sequence's u, times sum(w) until pref_finish_kernel has made the scale
+	float* coef;          // [2 n]: gradient of sum_i w_i l_i to a sequence's u
 	double* each;         // [2][n]: w l, w z
+	double* total;        // device scalar: sum(w)
 	float* scale;         // device scalar: grad_scale / sum(w)
 	float* stats;         // [3]: loss, mean margin, sum(w)
 };
-__device__ __forceinline__ void pref_pair(const Pref& g, int i, double up, double un) {
-	const double z = g.beta * (up - un), w = g.weight ? (double)g.weight[i] : 1.0;
-	double l, dz;
+__device__ __forceinline__ double pref_margin(const Pref& g, double up, double un) { return g.beta * (up - un); }
+__device__ __forceinline__ float pref_weight(const Pref& g, int i) { return g.weight ? g.weight[i] : 1.f; }
+// gradient of sum_i w_i l_i to u of pair i's preferred sequence (the other's is its negative): a sigmoid's small side is formed by itself, without a difference
+__device__ __forceinline__ float pref_slope(const Pref& g, int i, double z) {
+	float dz;
+	if (g.kind == NOVIC_PREF_SIGMOID) {
+		const float e = expf(-fabsf((float)z)), small = e / (1.f + e), large = 1.f / (1.f + e);
+		const float at = z < 0.0 ? small : large, rest = z < 0.0 ? large : small;  // sigmoid(z), sigmoid(-z)
+		dz = (float)g.smoothing * at - (1.f - (float)g.smoothing) * rest;
+	} else if (g.kind == NOVIC_PREF_HINGE) {
+		dz = z < 1.0 ? -1.f : (z >= 1.0 ? 0.f : (float)z);  // (a NaN stays one)
+	} else {
+		dz = (float)(2.0 * (z - 0.5) / (g.beta * g.beta));
+	}
+	return pref_weight(g, i) * dz * (float)g.beta;
+}
+__device__ __forceinline__ void pref_terms(const Pref& g, int i, double z) {
+	double l;
 	if (g.kind == NOVIC_PREF_SIGMOID) {
 		const double soft = log1p(exp(-fabs(z)));  // -log sigmoid(z) = soft + max(-z, 0)
 		l = (1.0 - g.smoothing) * (soft + fmax(-z, 0.0)) + g.smoothing * (soft + fmax(z, 0.0));
-		dz = 1.0 / (1.0 + exp(-z)) - (1.0 - g.smoothing);
 	} else if (g.kind == NOVIC_PREF_HINGE) {
-		l = z < 1.0 ? 1.0 - z : (z >= 1.0 ? 0.0 : z);  // (a NaN stays one)
-		dz = z < 1.0 ? -1.0 : (z >= 1.0 ? 0.0 : z);
+		l = z < 1.0 ? 1.0 - z : (z >= 1.0 ? 0.0 : z);
 	} else {
 		const double u = (z - 0.5) / g.beta;
 		l = u * u;
-		dz = 2.0 * u / g.beta;
 	}
+	const double w = (double)pref_weight(g, i);
 	if (g.margin) g.margin[i] = (float)z;
-	const float c = (float)(w * dz * g.beta);
-	g.coef[i] = c;
-	g.coef[g.n + i] = -c;
 	g.each[i] = w * l;
 	g.each[g.n + i] = w * z;
 }
 // sum of one sequence's T values by `lanes` consecutive lanes (a power of two up to 64), in a fixed order
 __device__ __forceinline__ double seq_sum(const double* v, int T, int lane, int lanes) {
 	double u = 0.0;
-	for (int t = lane; t < T; t += lanes) u += v[t];
+	for (int t0 = lane; t0 < T; t0 += 8 * lanes) {  // eight values a lane requested at once
+		double part[8];
+#pragma unroll
+		for (int k = 0; k < 8; ++k) part[k] = v[min(t0 + k * lanes, T - 1)];
+#pragma unroll
+		for (int k = 0; k < 8; ++k) u += t0 + k * lanes < T ? part[k] : 0.0;
+	}
 	for (int o = lanes / 2; o > 0; o >>= 1) u += __shfl_xor(u, o, 64);
 	return u;
-}
-__global__ __launch_bounds__(256) void pref_pair_kernel(const Pref g, int lanes) {
-	const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) / lanes;
-	const int lane = threadIdx.x % lanes;
-	if (id >= g.n) return;
-	const int i = (int)id;
-	const double up = seq_sum(g.diff + (long long)i * g.T, g.T, lane, lanes), un = seq_sum(g.diff + ((long long)g.n + i) * g.T, g.T, lane, lanes);
-	if (lane == 0) pref_pair(g, i, up, un);
 }
 // three sums over a workgroup of 1024 in a fixed order; thread 0 has them
 __device__ __forceinline__ void sum3_1024(double& a, double& b, double& c, double* red) {
@@ -326,21 +376,218 @@ __device__ __forceinline__ void sum3_1024(double& a, double& b, double& c, doubl
 		}
 	}
 }
-__global__ __launch_bounds__(1024) void pref_finish_kernel(const Pref g) {
+// what a mean over the weights w sums to: the scale of the gradients and, from the sums of w l and w z, the three numbers of a call
+__device__ __forceinline__ float pref_scale(const Pref& g, double w) { return w != 0.0 ? (float)(g.grad_scale / w) : 0.f; }  // (no weight at all: no loss and no gradient)
+__device__ __forceinline__ void pref_stats(const Pref& g, double l, double z, double w) {
+	g.stats[0] = w != 0.0 ? (float)(l / w) : 0.f;
+	g.stats[1] = w != 0.0 ? (float)(z / w) : 0.f;
+	g.stats[2] = (float)w;
+}
+// all pairs, by one workgroup: the sums over the sequences, the pairs' terms and their coefficients, the three numbers
+__global__ __launch_bounds__(1024) void pref_all_kernel(const Pref g, int lanes) {
 	__shared__ double red[48];
+	const int lane = threadIdx.x % lanes, teams = 1024 / lanes;
 	double l = 0.0, z = 0.0, w = 0.0;
-	for (int i = threadIdx.x; i < g.n; i += 1024) {
-		l += g.each[i];
-		z += g.each[g.n + i];
-		w += g.weight ? (double)g.weight[i] : 1.0;
+	for (int i = threadIdx.x / lanes; i < g.n; i += teams) {
+		const double up = seq_sum(g.diff + (long long)i * g.T, g.T, lane, lanes), un = seq_sum(g.diff + ((long long)g.n + i) * g.T, g.T, lane, lanes);
+		if (lane == 0) {
+			const double m = pref_margin(g, up, un);
+			const float c = pref_slope(g, i, m);
+			pref_terms(g, i, m);
+			g.coef[i] = c;
+			g.coef[g.n + i] = -c;
+			l += g.each[i];
+			z += g.each[g.n + i];
+			w += (double)pref_weight(g, i);
+		}
 	}
 	sum3_1024(l, z, w, red);
 	if (threadIdx.x == 0) {
-		const bool any = w != 0.0;  // (no weight at all: no loss and no gradient)
-		g.stats[0] = any ? (float)(l / w) : 0.f;
-		g.stats[1] = any ? (float)(z / w) : 0.f;
-		g.stats[2] = (float)w;
-		*g.scale = any ? (float)(g.grad_scale / w) : 0.f;
+		pref_stats(g, l, z, w);
+		*g.scale = pref_scale(g, w);
+	}
+}
+// sum of the weights, for the form that makes gradients pair by pair
+__global__ __launch_bounds__(1024) void pref_weight_kernel(const Pref g) {
+	__shared__ double red[48];
+	double w = 0.0, a = 0.0, b = 0.0;
+	for (int i = threadIdx.x; i < g.n; i += 1024) w += (double)g.weight[i];
+	sum3_1024(w, a, b, red);
+	if (threadIdx.x == 0) *g.total = w;
+}
+__global__ __launch_bounds__(1024) void pref_finish_kernel(const Pref g) {
+	__shared__ double red[48];
+	double l = 0.0, z = 0.0, none = 0.0;
+	for (int i = threadIdx.x; i < g.n; i += 1024) {
+		l += g.each[i];
+		z += g.each[g.n + i];
+	}
+	sum3_1024(l, z, none, red);
+	if (threadIdx.x == 0) pref_stats(g, l, z, g.weight ? *g.total : (double)g.n);
+}
+
+// A row in the registers of a wave, as it lies in memory.  Vector c of all lanes together is the STEP elements from c STEP on; where those would leave the row it is the row's
+// last STEP elements, of which the first cut(c) belong to vectors before it: a scalar base and one offset a lane address everything, and no load is conditional (a conditional
+// one in a loop costs a second copy of the registers).  NC = 1: a row of at most STEP elements, each lane's vector moved back by itself.
+template <typename T, int CH, int NC>
+struct WaveRow {
+	static constexpr int STEP = 64 * CH;
+	RawVec<T, CH> raw[NC];
+	__device__ __forceinline__ static int base(int c, int V) { return NC == 1 ? 0 : min(c * STEP, V - STEP); }
+	__device__ __forceinline__ static int at(int V, int lane) { return NC == 1 ? min(lane * CH, V - CH) : lane * CH; }
+	__device__ __forceinline__ static int cut(int c, int V, int lane) { return NC == 1 ? lane * CH : c * STEP - base(c, V); }  // first element of at() .. that counts
+	__device__ __forceinline__ static bool whole(int c, int V) { return (c + 1) * STEP <= V; }
+	__device__ __forceinline__ static bool any(int c, int V) { return c * STEP < V; }
+	__device__ __forceinline__ void load(const T* row, int V, int lane) {
+#pragma unroll
+		for (int c = 0; c < NC; ++c) raw[c] = load_vec<T, CH>(elem(row + base(c, V), at(V, lane)));
+	}
+	// The maximum of 16-bit elements two at a time, as integers: a number that is not negative compares as its bits do, and above every negative one.  Only a row whose maximum
+	// comes out negative is looked over again, element by element (there the bits of the lowest number win).
+	__device__ __forceinline__ float top() {
+		float t = -INFINITY;
+		if constexpr (sizeof(T) == 2 && CH > 1) {
+			typedef short pair __attribute__((ext_vector_type(2)));
+			pair best = {(short)0x8000, (short)0x8000};
+#pragma unroll
+			for (int c = 0; c < NC; ++c)
+#pragma unroll
+				for (int i = 0; i < CH / 2; ++i) {
+					pair p;
+					__builtin_memcpy(&p, &raw[c].w[i], 4);
+					best = __builtin_elementwise_max(best, p);
+				}
+			RawVec<T, 2> r;
+			__builtin_memcpy(&r, &best, 4);
+			t = wave_max(fmaxf(r.get(0), r.get(1)));
+			if (t > 0.f) return t;
+			t = -INFINITY;
+		}
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+#pragma unroll
+			for (int i = 0; i < CH; ++i) t = fmaxf(t, raw[c].get(i));
+			forget(raw[c]);
+		}
+		return wave_max(t);
+	}
+	__device__ __forceinline__ void sum(int V, int lane, float& M, float& s) {
+		M = point(top());
+		float t = 0.f;
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+			forget(raw[c]);  // (else its elements stay unpacked from one use to the next, at twice the registers)
+			if (whole(c, V)) {
+#pragma unroll
+				for (int i = 0; i < CH; ++i) t += expo(raw[c].get(i), M);
+			} else if (any(c, V)) {
+#pragma unroll
+				for (int i = 0; i < CH; ++i) t += at(V, lane) + i >= cut(c, V, lane) ? expo(raw[c].get(i), M) : 0.f;
+			}
+		}
+		s = wave_sum(t);
+	}
+	__device__ __forceinline__ void grad(T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+			if (!any(c, V)) continue;
+			forget(raw[c]);
+			float o[CH];
+#pragma unroll
+			for (int i = 0; i < CH; ++i) o[i] = k * expo(raw[c].get(i), M);
+			if (whole(c, V)) {
+				store_vec<true>(elem(out + base(c, V), at(V, lane)), o);
+			} else if (at(V, lane) >= cut(c, V, lane)) {
+				store_vec<true>(elem(out + base(c, V), at(V, lane)), o);
+			} else {
+#pragma unroll
+				for (int i = 1; i < CH; ++i)
+					if (at(V, lane) + i >= cut(c, V, lane) && cut(c, V, lane) < V) *elem(out + base(c, V), at(V, lane) + i) = (T)o[i];
+			}
+		}
+		if (owner(target, V) == lane) out[target] = (T)(k * expo(xt, M) + coef);
+	}
+	// the lane that stores element v (after which it may store it once more)
+	__device__ __forceinline__ static int owner(int v, int V) {
+		if (NC == 1) return v / CH;
+		return v / STEP * STEP <= V - STEP ? v % STEP / CH : (v - (V - STEP)) / CH;
+	}
+};
+
+// A pair by one workgroup, loss and gradient.  The pair's rows (at most 64) are lanes' business first: each wave asks for all targets and reference values and knows the rows that
+// count from a ballot.  Those are dealt to the waves in turn; the row that a wave sums last stays in its registers up to its gradient, any others are read again (a pair's
+// time later: out of L2 or the memory-side cache).  Sixteen vectors a lane are what 128 registers hold beside the rest of the kernel.
+#ifndef PW
+#define PW 8
+#endif
+constexpr int PAIR_WAVES = PW, PAIR_ROWS = 64, PAIR_VECTORS = 16;
+template <typename T, int CH, int NC>
+__global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Rows g, const LogpOut o, const Pref q) {
+	__shared__ double part[2][PAIR_WAVES];
+	const int i = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, rows = 2 * q.T;
+	const int my_half = lane >= q.T, my_a = my_half ? q.n + i : i, my_t = lane - my_half * q.T;  // lane k stands for row k: the preferred sequence's, then the other's
+	int my_target = -1;
+	float my_ref = 0.f;
+	if (lane < rows) {
+		my_target = counted_target(g, my_a, my_t);
+		my_ref = o.ref[my_a * o.ldref + my_t];
+	}
+	const unsigned long long counted = __ballot(my_target >= 0), others = __ballot(lane < rows && my_target < 0);
+	const int have = __popcll(counted), none = __popcll(others);
+	auto nth = [&](unsigned long long set, int l) {  // the l-th member of a set of lanes
+		return __ffsll((unsigned long long)__ballot(((set >> lane) & 1) && __popcll(set & ((1ull << lane) - 1)) == l)) - 1;
+	};
+	auto row_of = [&](int k) { return (k >= q.T ? q.n + i : i) * q.T + (k >= q.T ? k - q.T : k); };
+	auto of_lane = [&](int v, int k) { return __builtin_amdgcn_readlane(v, k); };
+	double u[2] = {0.0, 0.0};
+	auto counted_row = [&](int k, int r, float xt, float M, float s) {  // lane 0: the row's log-probability, added to its sequence
+		const double lp = row_logp(xt, M, s), d = lp - (double)__int_as_float(of_lane(__float_as_int(my_ref), k));
+		u[0] += k >= q.T ? 0.0 : d;
+		u[1] += k >= q.T ? d : 0.0;
+		if (lane == 0) put_logp(o, r, k >= q.T ? q.n + i : i, k >= q.T ? k - q.T : k, true, lp, M, s);
+	};
+	WaveRow<T, CH, NC> tile;
+	float M = 0.f, s = 1.f, xt = 0.f;
+	int k = 0, r = 0, target = 0;
+	for (int l = wave + (have - 1 - wave) / PAIR_WAVES * PAIR_WAVES; wave < have && l >= 0; l -= PAIR_WAVES) {
+		k = nth(counted, l), r = row_of(k), target = of_lane(my_target, k);
+		const T* row = (const T*)g.logits + (long long)r * g.ldl;
+		tile.load(row, g.V, lane);
+		xt = (float)row[target];
+		tile.sum(g.V, lane, M, s);
+		counted_row(k, r, xt, M, s);
+	}
+	if (lane == 0) {
+		part[0][wave] = u[0];
+		part[1][wave] = u[1];
+	}
+	for (int l = PAIR_WAVES - 1 - wave; l < none; l += PAIR_WAVES) {
+		const int kz = nth(others, l), rz = row_of(kz);
+		if (g.dlogits) RowStream<T, CH, 64>::zero((T*)g.dlogits + (long long)rz * g.ldd, g.V, lane);
+		if (lane == 0) put_logp(o, rz, kz >= q.T ? q.n + i : i, kz >= q.T ? kz - q.T : kz, false, 0.0, 0.f, 1.f);
+	}
+	__syncthreads();
+	u[0] = u[1] = 0.0;
+#pragma unroll
+	for (int w = 0; w < PAIR_WAVES; ++w) {
+		u[0] += part[0][w];
+		u[1] += part[1][w];
+	}
+	const double z = pref_margin(q, u[0], u[1]);
+	if (threadIdx.x == PAIR_WAVES * 64 - 1) pref_terms(q, i, z);  // (the last wave: it has the fewest rows)
+	if (!g.dlogits) return;
+	const float c = pref_slope(q, i, z) * pref_scale(q, q.weight ? *q.total : (double)q.n);
+	if (wave >= have) return;
+	float coef = k >= q.T ? -c : c;
+	tile.grad((T*)g.dlogits + (long long)r * g.ldd, g.V, lane, target, xt, M, -coef / s, coef);
+	for (int l = wave + PAIR_WAVES; l < have; l += PAIR_WAVES) {
+		k = nth(counted, l), r = row_of(k), target = of_lane(my_target, k);
+		const T* row = (const T*)g.logits + (long long)r * g.ldl;
+		const float2 norm = o.norm[r];  // (written by this wave)
+		tile.load(row, g.V, lane);
+		xt = (float)row[target];
+		coef = k >= q.T ? -c : c;
+		tile.grad((T*)g.dlogits + (long long)r * g.ldd, g.V, lane, target, xt, norm.x, -coef * norm.y, coef);
 	}
 }
 
@@ -355,7 +602,8 @@ struct Policy {
 	int* len;          // [A]: counted rows of a sequence
 	int* part;         // [2][parts]: counted rows, sequences with any, of the sequences of one block of policy_count_kernel
 	int parts;
-	float* each;       // [3][A T]: loss, KL, clipped, each times the row's share of the mean
+	float4* each;      // [A T]: loss, KL, clipped, each times the row's share of the mean
+	double* slices;    // [64][3]: sums over the slices of policy_finish_kernel
 	float* stats;      // [4]: loss, mean KL, clipped share, counted rows
 };
 __global__ __launch_bounds__(256) void policy_count_kernel(const Rows g, const Policy p, int lanes) {
@@ -416,17 +664,14 @@ __device__ __forceinline__ float policy_share(const Rows& g, const Policy& p, in
 }
 // what one thread of the row writes: its log-probability and its terms of the means
 __device__ __forceinline__ void policy_put(const Rows& g, const Policy& p, int r, int a, int t, double lp, float share, const PolicyRow& w) {
-	const long long R = (long long)g.A * g.T;
 	const double kl = p.ref ? expm1(w.d) - w.d : 0.0;
 	if (p.logp) p.logp[a * p.ldo + t] = (float)lp;
-	p.each[r] = (float)(((w.whole ? -(double)w.q * w.adv : -(double)w.held * w.adv) + (double)p.kl_coef * kl) * share);
-	p.each[R + r] = (float)(kl * share);
-	p.each[2 * R + r] = w.whole ? 0.f : share;
+	const double l = (w.whole ? -(double)w.q * w.adv : -(double)w.held * w.adv) + (double)p.kl_coef * kl;
+	p.each[r] = make_float4((float)(l * share), (float)(kl * share), w.whole ? 0.f : share, 0.f);
 }
 __device__ __forceinline__ void policy_put_none(const Rows& g, const Policy& p, int r, int a, int t) {
-	const long long R = (long long)g.A * g.T;
 	if (p.logp) p.logp[a * p.ldo + t] = 0.f;
-	p.each[r] = p.each[R + r] = p.each[2 * R + r] = 0.f;
+	p.each[r] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 template <typename T, int CH, int THREADS, int NC>
 __global__ __launch_bounds__(THREADS) void policy_kernel(const Rows g, const Policy p) {
@@ -437,7 +682,7 @@ __global__ __launch_bounds__(THREADS) void policy_kernel(const Rows g, const Pol
 	const int target = counted_target(g, a, t);
 	T* out = (T*)g.dlogits + (long long)r * g.ldd;
 	if (target < 0) {
-		if (g.dlogits) zero_row<T, CH, THREADS>(out, g.V);
+		if (g.dlogits) RowStream<T, CH, THREADS>::zero(out, g.V, threadIdx.x);
 		if (threadIdx.x == 0) policy_put_none(g, p, r, a, t);
 		return;
 	}
@@ -446,11 +691,11 @@ __global__ __launch_bounds__(THREADS) void policy_kernel(const Rows g, const Pol
 	tile.load(row, g.V);
 	const float xt = (float)row[target], share = policy_share(g, p, a);
 	tile.sum(g.V, red);
-	const double lp = ((double)xt - (double)tile.m) - log_wide(tile.s);
+	const double lp = row_logp(xt, tile.M, tile.s);
 	PolicyRow w;
 	const float coef = policy_grad(p, a, t, lp, share, w);
 	if (threadIdx.x == 0) policy_put(g, p, r, a, t, lp, share, w);
-	if (g.dlogits) tile.grad(out, g.V, target, coef);
+	if (g.dlogits) tile.grad(out, g.V, target, expo(xt, tile.M), coef);
 }
 template <typename T, int CH, int THREADS>
 __global__ __launch_bounds__(THREADS) void policy_long_kernel(const Rows g, const Policy p) {
@@ -461,46 +706,64 @@ __global__ __launch_bounds__(THREADS) void policy_long_kernel(const Rows g, cons
 	const int target = counted_target(g, a, t);
 	T* out = (T*)g.dlogits + (long long)r * g.ldd;
 	if (target < 0) {
-		if (g.dlogits) zero_row<T, CH, THREADS>(out, g.V);
+		if (g.dlogits) RowStream<T, CH, THREADS>::zero(out, g.V, threadIdx.x);
 		if (threadIdx.x == 0) policy_put_none(g, p, r, a, t);
 		return;
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
 	const float xt = (float)row[target], share = policy_share(g, p, a);
-	float m, s;
-	long_row_sum<T, CH, THREADS>(row, g.V, red, m, s);
-	const double lp = ((double)xt - (double)m) - log_wide(s);
+	float M, s;
+	block_row_sum<T, CH, THREADS>(row, g.V, red, M, s);
+	const double lp = row_logp(xt, M, s);
 	PolicyRow w;
 	const float coef = policy_grad(p, a, t, lp, share, w);
 	if (threadIdx.x == 0) policy_put(g, p, r, a, t, lp, share, w);
-	if (!g.dlogits) return;
-	const float k = -coef / s;
-	for (int e0 = threadIdx.x * CH; e0 < g.V; e0 += THREADS * CH) {
-		const int es = min(e0, g.V - CH);
-		const RawVec<T, CH> raw = load_vec<T, CH>(elem(row, es));
-		float o[CH];
-#pragma unroll
-		for (int i = 0; i < CH; ++i) o[i] = (k * __builtin_amdgcn_exp2f((raw.get(i) - m) * LOG2E) + (es + i == target ? coef : 0.f));
-		store_own<T, CH>(out, es, e0, o);
-	}
+	if (g.dlogits) RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, M, -coef / s, coef);
 }
+// the sums over a slice of the rows, by workgroup; a second launch adds the slices, unless there is only one
 __global__ __launch_bounds__(1024) void policy_finish_kernel(const Rows g, const Policy p) {
 	__shared__ double red[48];
-	const long long R = (long long)g.A * g.T;
+	const long long R = (long long)g.A * g.T, slice = (R + gridDim.x - 1) / gridDim.x, first = blockIdx.x * slice, end = min(first + slice, R);
 	double l = 0.0, k = 0.0, c = 0.0;
-	for (long long r = threadIdx.x; r < R; r += 1024) {
-		l += (double)p.each[r];
-		k += (double)p.each[R + r];
-		c += (double)p.each[2 * R + r];
+	for (long long r0 = first + threadIdx.x; r0 < end; r0 += 8 * 1024) {  // eight rows a thread requested at once
+		float4 v[8];
+#pragma unroll
+		for (int i = 0; i < 8; ++i) v[i] = p.each[min(r0 + i * 1024, end - 1)];
+#pragma unroll
+		for (int i = 0; i < 8; ++i) {
+			if (r0 + i * 1024 >= end) continue;
+			l += (double)v[i].x;
+			k += (double)v[i].y;
+			c += (double)v[i].z;
+		}
 	}
 	sum3_1024(l, k, c, red);
-	const int n = policy_total(p, 0);
+	const int n = gridDim.x == 1 ? policy_total(p, 0) : 0;
 	if (threadIdx.x == 0) {
-		p.stats[0] = (float)l;
-		p.stats[1] = (float)k;
-		p.stats[2] = (float)c;
-		p.stats[3] = (float)n;
+		if (gridDim.x == 1) {
+			p.stats[0] = (float)l;
+			p.stats[1] = (float)k;
+			p.stats[2] = (float)c;
+			p.stats[3] = (float)n;
+		} else {
+			p.slices[3 * blockIdx.x] = l;
+			p.slices[3 * blockIdx.x + 1] = k;
+			p.slices[3 * blockIdx.x + 2] = c;
+		}
 	}
+}
+__global__ __launch_bounds__(64) void policy_slices_kernel(const Policy p) {
+	const int lane = threadIdx.x;
+	double v[3];
+#pragma unroll
+	for (int i = 0; i < 3; ++i) {
+		v[i] = p.slices[3 * lane + i];
+#pragma unroll
+		for (int o = 32; o > 0; o >>= 1) v[i] += __shfl_xor(v[i], o, 64);
+	}
+	const int n = policy_total(p, 0);
+	if (lane < 3) p.stats[lane] = (float)(lane == 0 ? v[0] : lane == 1 ? v[1] : v[2]);
+	if (lane == 3) p.stats[3] = (float)n;
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------------------------------------
@@ -520,17 +783,31 @@ dim3 rows_grid(const Rows& g) {
 	const long long R = (long long)g.A * g.T, x = std::min<long long>(R, 1 << 20);
 	return dim3((unsigned)x, (unsigned)((R + x - 1) / x));
 }
+// A team of a wave for rows that it takes in one go; else 256 lanes, or 1024 where there are too few rows to fill the chip with 256 (a row's own latency counts then).
+int row_threads(const Rows& g, int ch) { return g.V <= 64 * ch * 2 ? 64 : (long long)g.A * g.T < 1024 && g.V > 1024 * ch ? 1024 : 256; }
 template <typename T, int CH>
 void launch_logp(const Rows& g, const LogpOut& o, hipStream_t stream) {
 	const dim3 grid = rows_grid(g);
-	NOVIC_ROW_SHAPES(g.V, (logp_kernel<T, CH, TH, NC><<<grid, dim3(TH), 0, stream>>>(g, o)),
-	                 (logp_long_kernel<T, CH, TH><<<grid, dim3(TH), 0, stream>>>(g, o)))
+	if constexpr (CH == 1) {
+		logp_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, o);
+	} else {
+		const int threads = row_threads(g, CH);
+		if (threads == 64) logp_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, o);
+		else if (threads == 256) logp_kernel<T, CH, 256><<<grid, dim3(256), 0, stream>>>(g, o);
+		else logp_kernel<T, CH, 1024><<<grid, dim3(1024), 0, stream>>>(g, o);
+	}
 }
 template <typename T, int CH>
 void launch_grad(const Rows& g, const GradIn& in, hipStream_t stream) {
 	const dim3 grid = rows_grid(g);
-	if (CH == 1 || g.V <= 64 * CH) logp_grad_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, in);
-	else logp_grad_kernel<T, CH, 256><<<grid, dim3(256), 0, stream>>>(g, in);
+	if constexpr (CH == 1) {
+		logp_grad_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, in);
+	} else {
+		const int threads = row_threads(g, CH);
+		if (threads == 64) logp_grad_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, in);
+		else if (threads == 256) logp_grad_kernel<T, CH, 256><<<grid, dim3(256), 0, stream>>>(g, in);
+		else logp_grad_kernel<T, CH, 1024><<<grid, dim3(1024), 0, stream>>>(g, in);
+	}
 }
 template <typename T, int CH>
 void launch_policy(const Rows& g, const Policy& p, hipStream_t stream) {
@@ -567,7 +844,7 @@ int lanes_for(int T) {
 	return lanes;
 }
 uint64_t up16(uint64_t n) { return (n + 15) / 16 * 16; }
-constexpr int COUNT_PARTS = 64;
+constexpr int COUNT_PARTS = 64, SLICES = 64;  // (one wave adds the parts)
 int count_parts(int A, int T) { return (int)std::min<long long>(COUNT_PARTS, ((long long)A * lanes_for(T) + 255) / 256); }
 
 }  // namespace
@@ -604,11 +881,29 @@ extern "C" int novic_token_logprobs_bwd(const void* logits, int type, int64_t ld
 	return 0;
 }
 
-// workspace: diff [2n T] fp64, each [2][n] fp64, norm [2n T] float2, coef [2n], scale
+// Pair by pair where the pairs alone fill the chip (two workgroups of eight waves a unit) and a wave's registers hold a row; else row by row, with a launch over the pairs between
+// the two over the rows.
+constexpr int FUSED_PAIRS = 512;
+bool pair_by_pair(const Rows& g, int type) { return g.A / 2 >= FUSED_PAIRS && 2 * g.T <= PAIR_ROWS && g.V <= PAIR_VECTORS * 64 * (type == NOVIC_TYPE_F32 ? 4 : 8); }
+template <typename T, int CH>
+void launch_pairs(const Rows& g, const LogpOut& o, const Pref& q, hipStream_t stream) {
+	const dim3 grid((unsigned)q.n), block(PAIR_WAVES * 64);
+	if constexpr (CH == 1) {
+		pref_pair_kernel<T, CH, 1><<<grid, block, 0, stream>>>(g, o, q);
+	} else {
+		if (g.V <= 64 * CH) pref_pair_kernel<T, CH, 1><<<grid, block, 0, stream>>>(g, o, q);
+		else if (g.V <= 4 * 64 * CH) pref_pair_kernel<T, CH, 4><<<grid, block, 0, stream>>>(g, o, q);
+		else if (g.V <= 8 * 64 * CH) pref_pair_kernel<T, CH, 8><<<grid, block, 0, stream>>>(g, o, q);
+		else if (g.V <= 12 * 64 * CH) pref_pair_kernel<T, CH, 12><<<grid, block, 0, stream>>>(g, o, q);
+		else pref_pair_kernel<T, CH, PAIR_VECTORS><<<grid, block, 0, stream>>>(g, o, q);
+	}
+}
+
+// workspace: diff [2n T] fp64, each [2][n] fp64, norm [2n T] float2, coef [2n], total fp64, scale
 extern "C" uint64_t novic_preference_loss_ws(int n, int T) {
 	if (n <= 0 || T <= 0) return 0;
 	const uint64_t R = 2ull * n * T;
-	return up16(8 * R) + up16(16ull * n) + up16(8 * R) + up16(8ull * n) + 16;
+	return up16(8 * R) + up16(16ull * n) + up16(8 * R) + up16(8ull * n) + 32;
 }
 extern "C" int novic_preference_loss(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int n, int T, int V,
                                      const float* ref, int64_t ldref, const float* weight, int kind, double beta, double smoothing, double grad_scale, float* logp, int64_t ldo,
@@ -630,27 +925,32 @@ extern "C" int novic_preference_loss(const void* logits, int type, int64_t ldl, 
 	double* each = (double*)w; w += up16(16ull * n);
 	float2* norm = (float2*)w; w += up16(8 * R);
 	float* coef = (float*)w; w += up16(8ull * n);
-	float* scale = (float*)w;
+	double* total = (double*)w; w += 16;
 	LogpOut o = {};
-	o.logp = logp; o.ldo = ldo; o.ref = ref; o.ldref = ldref; o.diff = diff; o.norm = dlogits ? norm : nullptr;
-	NOVIC_ROW_TYPES(type, V, launch_logp, g, o, stream)
-	Pref q = {diff, weight, n, T, kind, beta, smoothing, grad_scale, margin, coef, each, scale, stats};
-	const int lanes = lanes_for(T);
-	pref_pair_kernel<<<dim3((unsigned)(((long long)n * lanes + 255) / 256)), dim3(256), 0, stream>>>(q, lanes);
-	pref_finish_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q);
-	if (dlogits) {
-		GradIn in = {};
-		in.norm = norm; in.grad = coef; in.lda = 1; in.ldt = 0; in.scale = scale;
-		NOVIC_ROW_TYPES(type, V, launch_grad, g, in, stream)
+	o.logp = logp; o.ldo = ldo; o.ref = ref; o.ldref = ldref; o.norm = dlogits ? norm : nullptr;
+	const Pref q = {diff, weight, n, T, kind, beta, smoothing, grad_scale, margin, coef, each, total, (float*)w, stats};
+	if (pair_by_pair(g, type)) {
+		if (weight) pref_weight_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q);
+		NOVIC_ROW_TYPES(type, V, launch_pairs, g, o, q, stream)
+		pref_finish_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q);
+	} else {
+		o.diff = diff;
+		NOVIC_ROW_TYPES(type, V, launch_logp, g, o, stream)
+		pref_all_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q, lanes_for(T));
+		if (dlogits) {
+			GradIn in = {};
+			in.norm = norm; in.grad = coef; in.lda = 1; in.ldt = 0; in.scale = q.scale;
+			NOVIC_ROW_TYPES(type, V, launch_grad, g, in, stream)
+		}
 	}
 	NOVIC_LAUNCH_CHECK();
 	return 0;
 }
 
-// workspace: len [A], part [2][64], each [3][A T]
+// workspace: len [A], part [2][64], slices [64][3] fp64, each [A T] float4
 extern "C" uint64_t novic_policy_loss_ws(int A, int T) {
 	if (A <= 0 || T <= 0) return 0;
-	return up16(4ull * A) + up16(8 * COUNT_PARTS) + 12ull * A * T;
+	return up16(4ull * A) + up16(8 * COUNT_PARTS) + 24 * SLICES + 16ull * A * T;
 }
 extern "C" int novic_policy_loss(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int A, int T, int V,
                                  const float* old_logp, int64_t ldold, const float* adv, int64_t adv_lda, int64_t adv_ldt, const float* ref, int64_t ldref, float clip_lo, float clip_hi,
@@ -676,12 +976,16 @@ extern "C" int novic_policy_loss(const void* logits, int type, int64_t ldl, cons
 	char* w = (char*)ws;
 	p.len = (int*)w; w += up16(4ull * A);
 	p.part = (int*)w; w += up16(8 * COUNT_PARTS);
-	p.each = (float*)w;
+	p.slices = (double*)w; w += 24 * SLICES;
+	p.each = (float4*)w;
 	p.parts = count_parts(A, T);
 	p.stats = stats;
 	policy_count_kernel<<<dim3(p.parts), dim3(256), 0, stream>>>(g, p, lanes_for(T));
 	NOVIC_ROW_TYPES(type, V, launch_policy, g, p, stream)
-	policy_finish_kernel<<<dim3(1), dim3(1024), 0, stream>>>(g, p);
+	// one workgroup reads its rows' terms at some 50 GB/s: beyond 8192 rows (a batch of loads a thread) 64 of them and one launch more are shorter
+	const bool sliced = (long long)A * T > 8192;
+	policy_finish_kernel<<<dim3(sliced ? SLICES : 1), dim3(1024), 0, stream>>>(g, p);
+	if (sliced) policy_slices_kernel<<<dim3(1), dim3(64), 0, stream>>>(p);
 	NOVIC_LAUNCH_CHECK();
 	return 0;
 }
