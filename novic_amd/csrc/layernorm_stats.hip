@@ -49,13 +49,18 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_fwd
 	}
 	const float inv = 1.f / (float)E;
 	const int stride = gridDim.x * TEAMS;
-	// (teams of more than a wave have a block of their own, so the rows of a block and with them the barriers in team_sum2 are the same for all its threads)
-	for (int row0 = blockIdx.x * TEAMS + team; row0 < rows; row0 += stride) {
-		const int row = LANES < 64 ? row0 : __builtin_amdgcn_readfirstlane(row0);
-		const XT* xr = x + (long long)row * ldx;
-		RawVec<XT, CH> raw[NC];
+	auto load = [&](RawVec<XT, CH> (&raw)[NC], int of) {
+		const int row = LANES < 64 ? of : __builtin_amdgcn_readfirstlane(of);  // (the same for a wave)
 #pragma unroll
-		for (int c = 0; c < NC; ++c) raw[c] = load_vec<XT, CH>(elem(xr, es[c]));
+		for (int c = 0; c < NC; ++c) raw[c] = load_once<XT, CH>(elem(x + (long long)row * ldx, es[c]));
+	};
+	RawVec<XT, CH> raw[NC], next[NC];
+	const int first = blockIdx.x * TEAMS + team;
+	if (first < rows) load(raw, first);
+	// (teams of more than a wave have a block of their own, so the rows of a block and with them the barriers in team_sum2 are the same for all its threads)
+	for (int row0 = first; row0 < rows; row0 += stride) {
+		const int row = LANES < 64 ? row0 : __builtin_amdgcn_readfirstlane(row0);
+		load(next, min(row0 + stride, rows - 1));  // requested before this row is reduced
 		float v[NC][CH], s = 0.f, q = 0.f, off = 0.f, none = 0.f;
 #pragma unroll
 		for (int c = 0; c < NC; ++c)
@@ -98,6 +103,8 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_fwd
 			}
 			store_own<false>(y + (long long)row * ldy, es[c], (c * LANES + lane) * CH, o);
 		}
+#pragma unroll
+		for (int c = 0; c < NC; ++c) raw[c] = next[c];
 	}
 }
 
@@ -135,9 +142,9 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_bwd
 		const int row = LANES < 64 ? of : __builtin_amdgcn_readfirstlane(of);  // (the same for a wave)
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
-			r.x[c] = load_vec<XT, CH>(elem(x + (long long)row * ldx, es[c]));
-			r.dy[c] = load_vec<YT, CH>(elem(dy + (long long)row * lddy, es[c]));
-			if (AHEAD && dx_in) r.in[c] = load_vec<XT, CH>(elem(dx_in + (long long)row * ldi, es[c]));
+			r.x[c] = load_once<XT, CH>(elem(x + (long long)row * ldx, es[c]));
+			r.dy[c] = load_once<YT, CH>(elem(dy + (long long)row * lddy, es[c]));
+			if (AHEAD && dx_in) r.in[c] = load_once<XT, CH>(elem(dx_in + (long long)row * ldi, es[c]));
 		}
 		r.mu = mean[row];
 		r.rs = rstd[row];
@@ -179,7 +186,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_bwd
 				asm volatile("" ::: "memory");
 				__builtin_amdgcn_sched_barrier(0);
 				gm[c] = load_vec<float, CH>(elem(gamma, es[c]));
-				if (dx_in) cur.in[c] = load_vec<XT, CH>(elem(dx_in + (long long)row * ldi, es[c]));
+				if (dx_in) cur.in[c] = load_once<XT, CH>(elem(dx_in + (long long)row * ldi, es[c]));
 			}
 			float o[CH];
 #pragma unroll
@@ -239,8 +246,13 @@ __global__ __launch_bounds__(1024) void layernorm_stats_reduce_kernel(const floa
 	if (!out) return;  // uniform over the block
 	const int col = threadIdx.x & 31, grp = threadIdx.x >> 5, e = blockIdx.x * 32 + col;
 	float t = 0.f;
-	if (e < E)
-		for (int r = grp; r < parts; r += 32) t += part[(long long)r * E + e];
+	for (int r0 = grp; e < E && r0 < parts; r0 += 8 * 32) {  // eight partial rows a thread requested at once
+		float v[8];
+#pragma unroll
+		for (int k = 0; k < 8; ++k) v[k] = part[(long long)min(r0 + k * 32, parts - 1) * E + e];
+#pragma unroll
+		for (int k = 0; k < 8; ++k) t += r0 + k * 32 < parts ? v[k] : 0.f;
+	}
 	sum[grp][col] = t;
 	__syncthreads();
 	if (grp == 0 && e < E) {
@@ -251,6 +263,9 @@ __global__ __launch_bounds__(1024) void layernorm_stats_reduce_kernel(const floa
 	}
 }
 
+#ifndef DIRECT
+#define DIRECT 4
+#endif
 struct Plan {
 	int lanes, chunks, blocks;
 };
@@ -260,7 +275,9 @@ Plan plan(int rows, int E, int ch, bool bwd) {
 	p.lanes = E <= 16 * ch ? 16 : E <= 256 * ch ? 64 : E <= 1024 * ch ? 256 : 512;
 	p.chunks = (E + p.lanes * ch - 1) / (p.lanes * ch);
 	const int teams = p.lanes > 256 ? 1 : 256 / p.lanes;
-	const int most = bwd ? (p.lanes > 256 ? 256 : 512) : 2048;
+	// Forward: four workgroups a unit (1024: 30.2 us, 2048: 31.8, 4096: 30.9 on [57344 x 512] fp32 -> bf16).  Backward: as many as are resident at once, two a unit, one of 512
+	// lanes: each leaves a partial row of both gradients behind.  A handful of rows is one workgroup's business, which needs no second launch.
+	const int most = !bwd ? 1024 : p.lanes > 256 ? 256 : rows <= DIRECT * teams ? 1 : 512;
 	p.blocks = (int)std::min<long long>(most, ((long long)rows + teams - 1) / teams);
 	return p;
 }

@@ -45,6 +45,24 @@ __device__ __forceinline__ RawVec<T, N> load_vec(const T* p) {
 	__builtin_memcpy(&r, p, sizeof(r));
 	return r;
 }
+// the same, for what the kernel reads once: the caches need not keep it
+template <typename T, int N>
+__device__ __forceinline__ RawVec<T, N> load_once(const T* p) {
+	RawVec<T, N> r;
+	if constexpr (sizeof(r) % 8 == 0) {
+		constexpr int W = sizeof(r) % 16 == 0 ? 4 : 2;
+		typedef uint32_t words __attribute__((ext_vector_type(W), aligned(2), may_alias));
+#pragma unroll
+		for (int i = 0; i < RawVec<T, N>::WORDS; i += W) {
+			const words q = __builtin_nontemporal_load((const words*)((const uint32_t*)p + i));
+#pragma unroll
+			for (int k = 0; k < W; ++k) r.w[i + k] = q[k];
+		}
+	} else {
+		__builtin_memcpy(&r, p, sizeof(r));
+	}
+	return r;
+}
 // element e of a row: the offset is 32 bits, so that a row that is the same for the wave keeps its address in scalar registers
 template <typename T>
 __device__ __forceinline__ T* elem(T* row, int e) {
@@ -54,13 +72,14 @@ template <typename T>
 __device__ __forceinline__ const T* elem(const T* row, int e) {
 	return (const T*)((const char*)row + (uint32_t)e * (uint32_t)sizeof(T));
 }
+// (The vectors of words may stand for elements of any type: an output may be an input, and no load may pass a store that changes what it reads.)
 // STREAM: past the caches (an output larger than they are, which nobody finds there again, leaves them to the inputs)
 template <bool STREAM, typename T, int N>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
 	RawVec<T, N> r;
 	r.put(f);
 	if constexpr (STREAM && sizeof(r) % 16 == 0) {
-		typedef uint32_t quad __attribute__((ext_vector_type(4), aligned(2)));
+		typedef uint32_t quad __attribute__((ext_vector_type(4), aligned(2), may_alias));
 #pragma unroll
 		for (int i = 0; i < (int)sizeof(r) / 16; ++i) {
 			const quad q = {r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
@@ -95,6 +114,12 @@ template <int LANES>
 __device__ __forceinline__ float team_sum(float v) {
 #pragma unroll
 	for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+	return v;
+}
+template <int LANES>
+__device__ __forceinline__ float team_max(float v) {
+#pragma unroll
+	for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
 	return v;
 }
 

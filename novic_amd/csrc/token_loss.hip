@@ -150,13 +150,14 @@ struct RowStream {
 			for (int u = 0; u < UNROLL; ++u) raw[u] = load_vec<T, CH>(elem(row, min(e + (u * LANES + lane) * CH, V - CH)));
 		}
 	}
-	// point and sum over this lane's part, with a running maximum
+	// point and sum over this lane's part, with a running maximum; the next vectors are requested before the present ones are added
 	__device__ __forceinline__ static void sum(const T* row, int V, int lane, float& tM, float& ts) {
 		tM = -INFINITY;
 		ts = 0.f;
+		RawVec<T, CH> raw[UNROLL], next[UNROLL];
+		load(raw, row, 0, V, lane);
 		for (int e = 0; e < V; e += UNROLL * LANES * CH) {
-			RawVec<T, CH> raw[UNROLL];
-			load(raw, row, e, V, lane);
+			if (e + UNROLL * LANES * CH < V) load(next, row, e + UNROLL * LANES * CH, V, lane);
 			float top = -INFINITY;
 #pragma unroll
 			for (int u = 0; u < UNROLL; ++u) {
@@ -180,6 +181,8 @@ struct RowStream {
 				}
 			}
 			tM = M;
+#pragma unroll
+			for (int u = 0; u < UNROLL; ++u) raw[u] = next[u];
 		}
 	}
 	// a lane's sum seen from the row's point
@@ -189,9 +192,10 @@ struct RowStream {
 	}
 	// out = k exp2(x log2 e - M), and coef more at the target (whose logit is xt); out may be row
 	__device__ __forceinline__ static void grad(const T* row, T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
+		RawVec<T, CH> raw[UNROLL], next[UNROLL];
+		load(raw, row, 0, V, lane);
 		for (int e = 0; e < V; e += UNROLL * LANES * CH) {
-			RawVec<T, CH> raw[UNROLL];
-			load(raw, row, e, V, lane);
+			if (e + UNROLL * LANES * CH < V) load(next, row, e + UNROLL * LANES * CH, V, lane);  // (before this piece's stores, also where out is row: no vector is in both)
 #pragma unroll
 			for (int u = 0; u < UNROLL; ++u) {
 				float o[CH];
@@ -204,6 +208,8 @@ struct RowStream {
 					if (e0 < V) store_own<true>(out, min(e0, V - CH), e0, o);
 				}
 			}
+#pragma unroll
+			for (int u = 0; u < UNROLL; ++u) raw[u] = next[u];
 		}
 		if ((target / CH) % LANES == lane) out[target] = (T)(k * expo(xt, M) + coef);
 	}
@@ -212,6 +218,122 @@ struct RowStream {
 #pragma unroll
 		for (int i = 0; i < CH; ++i) o[i] = 0.f;
 		for (int e0 = lane * CH; e0 < V; e0 += LANES * CH) store_own<true>(row, min(e0, V - CH), e0, o);
+	}
+};
+
+// A row in the registers of a team of LANES lanes (16 or 64), as it lies in memory.  Vector c of all lanes together is the STEP elements from c STEP on; where those would leave the row it is the row's
+// last STEP elements, of which the first cut(c) belong to vectors before it: a scalar base and one offset a lane address everything, and no load is conditional (a conditional
+// one in a loop costs a second copy of the registers).  NC = 1: a row of at most STEP elements, each lane's vector moved back by itself.
+template <typename T, int CH, int LANES, int NC>
+struct TeamRow {
+	static constexpr int STEP = LANES * CH;
+	RawVec<T, CH> raw[NC];
+	__device__ __forceinline__ static int base(int c, int V) { return NC == 1 ? 0 : min(c * STEP, V - STEP); }
+	__device__ __forceinline__ static int at(int V, int lane) { return NC == 1 ? min(lane * CH, V - CH) : lane * CH; }
+	__device__ __forceinline__ static int cut(int c, int V, int lane) { return NC == 1 ? lane * CH : c * STEP - base(c, V); }  // first element of at() .. that counts
+	__device__ __forceinline__ static bool whole(int c, int V) { return (c + 1) * STEP <= V; }
+	__device__ __forceinline__ static bool any(int c, int V) { return c * STEP < V; }
+	__device__ __forceinline__ void load(const T* row, int V, int lane) {
+#pragma unroll
+		for (int c = 0; c < NC; ++c) raw[c] = load_vec<T, CH>(elem(row + base(c, V), at(V, lane)));
+	}
+	// The maximum of 16-bit elements two at a time, as integers: a number that is not negative compares as its bits do, and above every negative one.  Only a row whose maximum
+	// comes out negative is looked over again, element by element (there the bits of the lowest number win).
+	__device__ __forceinline__ float top() {
+		float t = -INFINITY;
+		if constexpr (sizeof(T) == 2 && CH > 1) {
+			typedef short pair __attribute__((ext_vector_type(2)));
+			pair best = {(short)0x8000, (short)0x8000};
+#pragma unroll
+			for (int c = 0; c < NC; ++c)
+#pragma unroll
+				for (int i = 0; i < CH / 2; ++i) {
+					pair p;
+					__builtin_memcpy(&p, &raw[c].w[i], 4);
+					best = __builtin_elementwise_max(best, p);
+				}
+			RawVec<T, 2> r;
+			__builtin_memcpy(&r, &best, 4);
+			t = team_max<LANES>(fmaxf(r.get(0), r.get(1)));
+			if (t > 0.f) return t;
+			t = -INFINITY;
+		}
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+#pragma unroll
+			for (int i = 0; i < CH; ++i) t = fmaxf(t, raw[c].get(i));
+			forget(raw[c]);
+		}
+		return team_max<LANES>(t);
+	}
+	__device__ __forceinline__ void sum(int V, int lane, float& M, float& s) {
+		M = point(top());
+		float t = 0.f;
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+			forget(raw[c]);  // (else its elements stay unpacked from one use to the next, at twice the registers)
+			if (whole(c, V)) {
+#pragma unroll
+				for (int i = 0; i < CH; ++i) t += expo(raw[c].get(i), M);
+			} else if (any(c, V)) {
+#pragma unroll
+				for (int i = 0; i < CH; ++i) t += at(V, lane) + i >= cut(c, V, lane) ? expo(raw[c].get(i), M) : 0.f;
+			}
+		}
+		s = team_sum<LANES>(t);
+	}
+	__device__ __forceinline__ void grad(T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+			if (!any(c, V)) continue;
+			forget(raw[c]);
+			float o[CH];
+#pragma unroll
+			for (int i = 0; i < CH; ++i) o[i] = k * expo(raw[c].get(i), M);
+			if (whole(c, V)) {
+				store_vec<true>(elem(out + base(c, V), at(V, lane)), o);
+			} else if (at(V, lane) >= cut(c, V, lane)) {
+				store_vec<true>(elem(out + base(c, V), at(V, lane)), o);
+			} else {
+#pragma unroll
+				for (int i = 1; i < CH; ++i)
+					if (at(V, lane) + i >= cut(c, V, lane) && cut(c, V, lane) < V) *elem(out + base(c, V), at(V, lane) + i) = (T)o[i];
+			}
+		}
+		if (owner(target, V) == lane) out[target] = (T)(k * expo(xt, M) + coef);
+	}
+	// the lane that stores element v (after which it may store it once more)
+	__device__ __forceinline__ static int owner(int v, int V) {
+		if (NC == 1) return v / CH;
+		return v / STEP * STEP <= V - STEP ? v % STEP / CH : (v - (V - STEP)) / CH;
+	}
+};
+
+// Rows by team: the teams of a launch walk over the rows.  A row's mask and target are requested while the row before it is worked on, and looked at when its turn comes.
+template <int LANES>
+struct Walk {
+	int r, step, a, t;
+	bool padded;
+	long long id;
+	// (where a team is a wave, what is the same for it goes to scalar registers)
+	__device__ __forceinline__ static int same(int v) { return LANES == 64 ? __builtin_amdgcn_readfirstlane(v) : v; }
+	__device__ __forceinline__ Walk(const Rows& g) : r(same(blockIdx.x * (256 / LANES) + threadIdx.x / LANES)), step(gridDim.x * (256 / LANES)) { ask(g); }
+	__device__ __forceinline__ void ask(const Rows& g) {
+		a = r / g.T;
+		t = r - a * g.T;
+		padded = true;
+		id = -1;
+		if (done(g)) return;
+		padded = g.pad && g.pad[a * g.ldp + t];
+		id = g.tok_bytes == 8 ? ((const long long*)g.target)[a * g.ldt + t] : (long long)((const int*)g.target)[a * g.ldt + t];
+	}
+	__device__ __forceinline__ int target(const Rows& g) const { return same(padded || id < 0 || id >= g.V ? -1 : (int)id); }
+	__device__ __forceinline__ bool done(const Rows& g) const { return r >= g.A * g.T; }
+	__device__ __forceinline__ Walk next(const Rows& g) const {
+		Walk n = *this;
+		n.r = r > 0x7fffffff - step ? 0x7fffffff : r + step;
+		n.ask(g);
+		return n;
 	}
 };
 
@@ -258,6 +380,28 @@ __global__ __launch_bounds__(THREADS) void logp_kernel(const Rows g, const LogpO
 	if (threadIdx.x == 0) put_logp(o, r, a, t, true, row_logp(xt, M, s), M, s, ref);
 }
 
+template <typename T, int CH, int LANES, int NC>
+__global__ __launch_bounds__(256) void logp_team_kernel(const Rows g, const LogpOut o) {
+	const int lane = threadIdx.x % LANES;
+	TeamRow<T, CH, LANES, NC> tile;
+	Walk<LANES> now(g);
+	while (!now.done(g)) {
+		const int target = now.target(g);
+		float xt = 0.f, ref = 0.f;
+		if (target >= 0) {
+			const T* row = (const T*)g.logits + (long long)now.r * g.ldl;
+			tile.load(row, g.V, lane);
+			xt = (float)row[target];
+			ref = reference(o, now.a, now.t);
+		}
+		const Walk<LANES> next = now.next(g);
+		float M = 0.f, s = 1.f;
+		if (target >= 0) tile.sum(g.V, lane, M, s);
+		if (lane == 0) put_logp(o, now.r, now.a, now.t, target >= 0, target >= 0 ? row_logp(xt, M, s) : 0.0, M, s, ref);
+		now = next;
+	}
+}
+
 // ---- gradient of log-probabilities: dlogits = coef (1[v = target] - exp(x - m) / s) ----------------------------------------------------------------------------------
 struct GradIn {
 	const float* lse;     // [A T], or null:
@@ -266,6 +410,21 @@ struct GradIn {
 	long long lda, ldt;
 	const float* scale;   // device scalar or null
 };
+// dlogits = k exp2(x log2 e - M) + (coef at the target)
+__device__ __forceinline__ void grad_terms(const GradIn& in, int r, int a, int t, float& M, float& k, float& coef) {
+	coef = in.grad[a * in.lda + t * in.ldt];
+	if (in.scale) coef *= *in.scale;
+	k = -coef;
+	if (in.norm) {
+		const float2 n = in.norm[r];
+		M = n.x;
+		k *= n.y;
+	} else {
+		const float lse = in.lse[r];
+		M = point(lse);
+		k *= __builtin_amdgcn_exp2f(-fmaf(lse, LOG2E, -M));  // (what the point's rounding took: s is what lse says, seen from M)
+	}
+}
 template <typename T, int CH, int THREADS>
 __global__ __launch_bounds__(THREADS) void logp_grad_kernel(const Rows g, const GradIn in) {
 	const int r = row_index(g);
@@ -278,20 +437,31 @@ __global__ __launch_bounds__(THREADS) void logp_grad_kernel(const Rows g, const 
 		return;
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
-	float coef = in.grad[a * in.lda + t * in.ldt];
-	if (in.scale) coef *= *in.scale;
-	float M, k = -coef;
-	if (in.norm) {
-		const float2 n = in.norm[r];
-		M = n.x;
-		k *= n.y;
-	} else {
-		const float lse = in.lse[r];
-		M = point(lse);
-		k *= __builtin_amdgcn_exp2f(-fmaf(lse, LOG2E, -M));  // (what the point's rounding took: s is what lse says, seen from M)
-	}
+	float M, k, coef;
+	grad_terms(in, r, a, t, M, k, coef);
 	const float xt = (float)row[target];  // (used by the lane that owns the target alone, which loads it before it writes there: out may be row)
 	RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, M, k, coef);
+}
+
+template <typename T, int CH, int LANES>
+__global__ __launch_bounds__(256) void logp_grad_team_kernel(const Rows g, const GradIn in) {
+	typedef RowStream<T, CH, LANES> Stream;
+	const int lane = threadIdx.x % LANES;
+	Walk<LANES> now(g);
+	while (!now.done(g)) {
+		const int target = now.target(g);
+		T* out = (T*)g.dlogits + (long long)now.r * g.ldd;
+		const Walk<LANES> next = now.next(g);
+		if (target < 0) {
+			Stream::zero(out, g.V, lane);
+		} else {
+			float M, k, coef;
+			grad_terms(in, now.r, now.a, now.t, M, k, coef);
+			const T* row = (const T*)g.logits + (long long)now.r * g.ldl;
+			Stream::grad(row, out, g.V, lane, target, (float)row[target], M, k, coef);
+		}
+		now = next;
+	}
 }
 
 // ---- preference loss ---------------------------------------------------------------------------------------------------------------------------------------------
@@ -383,6 +553,18 @@ __device__ __forceinline__ void pref_stats(const Pref& g, double l, double z, do
 	g.stats[1] = w != 0.0 ? (float)(z / w) : 0.f;
 	g.stats[2] = (float)w;
 }
+// the pairs' terms and their coefficients by many workgroups; pref_finish_kernel adds the terms
+__global__ __launch_bounds__(256) void pref_each_kernel(const Pref g, int lanes) {
+	const int lane = threadIdx.x % lanes, i = (int)(((long long)blockIdx.x * 256 + threadIdx.x) / lanes);
+	if (i >= g.n) return;
+	const double up = seq_sum(g.diff + (long long)i * g.T, g.T, lane, lanes), un = seq_sum(g.diff + ((long long)g.n + i) * g.T, g.T, lane, lanes);
+	if (lane != 0) return;
+	const double m = pref_margin(g, up, un);
+	const float c = pref_slope(g, i, m);
+	pref_terms(g, i, m);
+	g.coef[i] = c;
+	g.coef[g.n + i] = -c;
+}
 // all pairs, by one workgroup: the sums over the sequences, the pairs' terms and their coefficients, the three numbers
 __global__ __launch_bounds__(1024) void pref_all_kernel(const Pref g, int lanes) {
 	__shared__ double red[48];
@@ -417,110 +599,36 @@ __global__ __launch_bounds__(1024) void pref_weight_kernel(const Pref g) {
 }
 __global__ __launch_bounds__(1024) void pref_finish_kernel(const Pref g) {
 	__shared__ double red[48];
-	double l = 0.0, z = 0.0, none = 0.0;
-	for (int i = threadIdx.x; i < g.n; i += 1024) {
-		l += g.each[i];
-		z += g.each[g.n + i];
+	double l = 0.0, z = 0.0, w = 0.0;
+	for (int i0 = threadIdx.x; i0 < g.n; i0 += 4 * 1024) {  // four pairs a thread requested at once
+		double a[4], b[4];
+		float c[4];
+#pragma unroll
+		for (int k = 0; k < 4; ++k) {
+			const int i = min(i0 + k * 1024, g.n - 1);
+			a[k] = g.each[i];
+			b[k] = g.each[g.n + i];
+			c[k] = pref_weight(g, i);
+		}
+#pragma unroll
+		for (int k = 0; k < 4; ++k) {
+			if (i0 + k * 1024 >= g.n) continue;
+			l += a[k];
+			z += b[k];
+			w += (double)c[k];
+		}
 	}
-	sum3_1024(l, z, none, red);
-	if (threadIdx.x == 0) pref_stats(g, l, z, g.weight ? *g.total : (double)g.n);
+	sum3_1024(l, z, w, red);
+	if (threadIdx.x == 0) {
+		pref_stats(g, l, z, w);
+		*g.scale = pref_scale(g, w);
+	}
 }
-
-// A row in the registers of a wave, as it lies in memory.  Vector c of all lanes together is the STEP elements from c STEP on; where those would leave the row it is the row's
-// last STEP elements, of which the first cut(c) belong to vectors before it: a scalar base and one offset a lane address everything, and no load is conditional (a conditional
-// one in a loop costs a second copy of the registers).  NC = 1: a row of at most STEP elements, each lane's vector moved back by itself.
-template <typename T, int CH, int NC>
-struct WaveRow {
-	static constexpr int STEP = 64 * CH;
-	RawVec<T, CH> raw[NC];
-	__device__ __forceinline__ static int base(int c, int V) { return NC == 1 ? 0 : min(c * STEP, V - STEP); }
-	__device__ __forceinline__ static int at(int V, int lane) { return NC == 1 ? min(lane * CH, V - CH) : lane * CH; }
-	__device__ __forceinline__ static int cut(int c, int V, int lane) { return NC == 1 ? lane * CH : c * STEP - base(c, V); }  // first element of at() .. that counts
-	__device__ __forceinline__ static bool whole(int c, int V) { return (c + 1) * STEP <= V; }
-	__device__ __forceinline__ static bool any(int c, int V) { return c * STEP < V; }
-	__device__ __forceinline__ void load(const T* row, int V, int lane) {
-#pragma unroll
-		for (int c = 0; c < NC; ++c) raw[c] = load_vec<T, CH>(elem(row + base(c, V), at(V, lane)));
-	}
-	// The maximum of 16-bit elements two at a time, as integers: a number that is not negative compares as its bits do, and above every negative one.  Only a row whose maximum
-	// comes out negative is looked over again, element by element (there the bits of the lowest number win).
-	__device__ __forceinline__ float top() {
-		float t = -INFINITY;
-		if constexpr (sizeof(T) == 2 && CH > 1) {
-			typedef short pair __attribute__((ext_vector_type(2)));
-			pair best = {(short)0x8000, (short)0x8000};
-#pragma unroll
-			for (int c = 0; c < NC; ++c)
-#pragma unroll
-				for (int i = 0; i < CH / 2; ++i) {
-					pair p;
-					__builtin_memcpy(&p, &raw[c].w[i], 4);
-					best = __builtin_elementwise_max(best, p);
-				}
-			RawVec<T, 2> r;
-			__builtin_memcpy(&r, &best, 4);
-			t = wave_max(fmaxf(r.get(0), r.get(1)));
-			if (t > 0.f) return t;
-			t = -INFINITY;
-		}
-#pragma unroll
-		for (int c = 0; c < NC; ++c) {
-#pragma unroll
-			for (int i = 0; i < CH; ++i) t = fmaxf(t, raw[c].get(i));
-			forget(raw[c]);
-		}
-		return wave_max(t);
-	}
-	__device__ __forceinline__ void sum(int V, int lane, float& M, float& s) {
-		M = point(top());
-		float t = 0.f;
-#pragma unroll
-		for (int c = 0; c < NC; ++c) {
-			forget(raw[c]);  // (else its elements stay unpacked from one use to the next, at twice the registers)
-			if (whole(c, V)) {
-#pragma unroll
-				for (int i = 0; i < CH; ++i) t += expo(raw[c].get(i), M);
-			} else if (any(c, V)) {
-#pragma unroll
-				for (int i = 0; i < CH; ++i) t += at(V, lane) + i >= cut(c, V, lane) ? expo(raw[c].get(i), M) : 0.f;
-			}
-		}
-		s = wave_sum(t);
-	}
-	__device__ __forceinline__ void grad(T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
-#pragma unroll
-		for (int c = 0; c < NC; ++c) {
-			if (!any(c, V)) continue;
-			forget(raw[c]);
-			float o[CH];
-#pragma unroll
-			for (int i = 0; i < CH; ++i) o[i] = k * expo(raw[c].get(i), M);
-			if (whole(c, V)) {
-				store_vec<true>(elem(out + base(c, V), at(V, lane)), o);
-			} else if (at(V, lane) >= cut(c, V, lane)) {
-				store_vec<true>(elem(out + base(c, V), at(V, lane)), o);
-			} else {
-#pragma unroll
-				for (int i = 1; i < CH; ++i)
-					if (at(V, lane) + i >= cut(c, V, lane) && cut(c, V, lane) < V) *elem(out + base(c, V), at(V, lane) + i) = (T)o[i];
-			}
-		}
-		if (owner(target, V) == lane) out[target] = (T)(k * expo(xt, M) + coef);
-	}
-	// the lane that stores element v (after which it may store it once more)
-	__device__ __forceinline__ static int owner(int v, int V) {
-		if (NC == 1) return v / CH;
-		return v / STEP * STEP <= V - STEP ? v % STEP / CH : (v - (V - STEP)) / CH;
-	}
-};
 
 // A pair by one workgroup, loss and gradient.  The pair's rows (at most 64) are lanes' business first: each wave asks for all targets and reference values and knows the rows that
 // count from a ballot.  Those are dealt to the waves in turn; the row that a wave sums last stays in its registers up to its gradient, any others are read again (a pair's
 // time later: out of L2 or the memory-side cache).  Sixteen vectors a lane are what 128 registers hold beside the rest of the kernel.
-#ifndef PW
-#define PW 8
-#endif
-constexpr int PAIR_WAVES = PW, PAIR_ROWS = 64, PAIR_VECTORS = 16;
+constexpr int PAIR_WAVES = 8, PAIR_ROWS = 64, PAIR_VECTORS = 16;
 template <typename T, int CH, int NC>
 __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Rows g, const LogpOut o, const Pref q) {
 	__shared__ double part[2][PAIR_WAVES];
@@ -546,7 +654,7 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 		u[1] += k >= q.T ? d : 0.0;
 		if (lane == 0) put_logp(o, r, k >= q.T ? q.n + i : i, k >= q.T ? k - q.T : k, true, lp, M, s);
 	};
-	WaveRow<T, CH, NC> tile;
+	TeamRow<T, CH, 64, NC> tile;
 	float M = 0.f, s = 1.f, xt = 0.f;
 	int k = 0, r = 0, target = 0;
 	for (int l = wave + (have - 1 - wave) / PAIR_WAVES * PAIR_WAVES; wave < have && l >= 0; l -= PAIR_WAVES) {
@@ -720,6 +828,39 @@ __global__ __launch_bounds__(THREADS) void policy_long_kernel(const Rows g, cons
 	if (threadIdx.x == 0) policy_put(g, p, r, a, t, lp, share, w);
 	if (g.dlogits) RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, M, -coef / s, coef);
 }
+template <typename T, int CH, int LANES, int NC>
+__global__ __launch_bounds__(256) void policy_team_kernel(const Rows g, const Policy p) {
+	const int lane = threadIdx.x % LANES;
+	TeamRow<T, CH, LANES, NC> tile;
+	Walk<LANES> now(g);
+	const int total = policy_total(p, p.per_seq ? 1 : 0);
+	while (!now.done(g)) {
+		const int target = now.target(g);
+		const bool counts = target >= 0;
+		const T* row = (const T*)g.logits + (long long)now.r * g.ldl;
+		T* out = (T*)g.dlogits + (long long)now.r * g.ldd;
+		float xt = 0.f, share = 0.f;
+		if (counts) {
+			tile.load(row, g.V, lane);
+			xt = (float)row[target];
+			share = p.per_seq ? 1.f / ((float)p.len[now.a] * (float)total) : 1.f / (float)total;
+		}
+		const Walk<LANES> next = now.next(g);
+		if (counts) {
+			float M, s;
+			tile.sum(g.V, lane, M, s);
+			const double lp = row_logp(xt, M, s);
+			PolicyRow w;
+			const float coef = policy_grad(p, now.a, now.t, lp, share, w);
+			if (g.dlogits) tile.grad(out, g.V, lane, target, xt, M, -coef / s, coef);
+			if (lane == 0) policy_put(g, p, now.r, now.a, now.t, lp, share, w);
+		} else {
+			if (g.dlogits) RowStream<T, CH, LANES>::zero(out, g.V, lane);
+			if (lane == 0) policy_put_none(g, p, now.r, now.a, now.t);
+		}
+		now = next;
+	}
+}
 // the sums over a slice of the rows, by workgroup; a second launch adds the slices, unless there is only one
 __global__ __launch_bounds__(1024) void policy_finish_kernel(const Rows g, const Policy p) {
 	__shared__ double red[48];
@@ -767,53 +908,66 @@ __global__ __launch_bounds__(64) void policy_slices_kernel(const Policy p) {
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------------------------------------
-// A register form holds threads * chunks vectors of CH elements; longer rows take the form that reads a row twice (its second pass comes out of L2 / the memory-side cache).
+// Rows in registers, by workgroup; longer ones take the form that reads a row twice (its second pass comes out of L2 / the memory-side cache).
 #define NOVIC_ROW_SHAPES(V, REG, LONG)                                                                     \
-	if constexpr (CH == 1) { constexpr int TH = 64, NC = 1; REG; } /* fewer than eight columns */             \
-	else if (V <= 64 * CH) { constexpr int TH = 64, NC = 1; REG; }                                           \
-	else if (V <= 256 * CH) { constexpr int TH = 256, NC = 1; REG; }                                         \
-	else if (V <= 512 * CH) { constexpr int TH = 256, NC = 2; REG; }                                         \
+	if (V <= 512 * CH) { constexpr int TH = 256, NC = 2; REG; }                                              \
 	else if (V <= 1024 * CH) { constexpr int TH = 256, NC = 4; REG; }                                        \
 	else if (V <= 2048 * CH) { constexpr int TH = 256, NC = 8; REG; }                                        \
 	else if (V <= 4096 * CH) { constexpr int TH = 1024, NC = 4; REG; }                                       \
 	else if (V <= 8192 * CH) { constexpr int TH = 1024, NC = 8; REG; }                                       \
 	else { constexpr int TH = 1024; LONG; }
+// Rows by team: sixteen lanes up to 64 CH columns, a wave with up to MOST vectors a lane beyond
+#define NOVIC_TEAM_SHAPES(V, MOST, CALL)                                                                   \
+	if (V <= 16 * CH) { constexpr int L = 16, NC = 1; CALL; }                                                \
+	else if (V <= 64 * CH) { constexpr int L = 16, NC = 4; CALL; }                                           \
+	else if (MOST == 4 || V <= 4 * 64 * CH) { constexpr int L = 64, NC = 4; CALL; }                          \
+	else if (V <= 8 * 64 * CH) { constexpr int L = 64, NC = MOST < 8 ? MOST : 8; CALL; }                     \
+	else { constexpr int L = 64, NC = MOST; CALL; }
 
+// Short rows go by team: a workgroup for each is mostly its own start and end ([104857 x 1500] bf16, log-probabilities 82 us by wave, 274 by workgroup; policy with gradient 158 and
+// 223; gradient 154 and 211).  Beyond four vectors a lane a workgroup's many registers win where there are gradients to store (4000 columns: 121 and 114 us); without, a wave
+// keeps up to sixteen, given rows enough for all waves (6000 columns: 64 and 84 us; at 1500 rows 9.1 and 8.1).
+template <int CH>
+bool by_team(const Rows& g, bool stores) { return g.V <= 4 * 64 * CH || (!stores && g.V <= 16 * 64 * CH && (long long)g.A * g.T >= 4096); }
+template <int LANES>
+dim3 team_grid(const Rows& g) { return dim3((unsigned)std::min<long long>(2048, ((long long)g.A * g.T + 256 / LANES - 1) / (256 / LANES))); }
 dim3 rows_grid(const Rows& g) {
 	const long long R = (long long)g.A * g.T, x = std::min<long long>(R, 1 << 20);
 	return dim3((unsigned)x, (unsigned)((R + x - 1) / x));
 }
-// A team of a wave for rows that it takes in one go; else 256 lanes, or 1024 where there are too few rows to fill the chip with 256 (a row's own latency counts then).
-int row_threads(const Rows& g, int ch) { return g.V <= 64 * ch * 2 ? 64 : (long long)g.A * g.T < 1024 && g.V > 1024 * ch ? 1024 : 256; }
 template <typename T, int CH>
 void launch_logp(const Rows& g, const LogpOut& o, hipStream_t stream) {
-	const dim3 grid = rows_grid(g);
 	if constexpr (CH == 1) {
-		logp_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, o);
+		logp_team_kernel<T, CH, 16, 1><<<team_grid<16>(g), dim3(256), 0, stream>>>(g, o);
+	} else if (by_team<CH>(g, false)) {
+		NOVIC_TEAM_SHAPES(g.V, 16, (logp_team_kernel<T, CH, L, NC><<<team_grid<L>(g), dim3(256), 0, stream>>>(g, o)))
 	} else {
-		const int threads = row_threads(g, CH);
-		if (threads == 64) logp_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, o);
-		else if (threads == 256) logp_kernel<T, CH, 256><<<grid, dim3(256), 0, stream>>>(g, o);
-		else logp_kernel<T, CH, 1024><<<grid, dim3(1024), 0, stream>>>(g, o);
+		logp_kernel<T, CH, 256><<<rows_grid(g), dim3(256), 0, stream>>>(g, o);
 	}
 }
+// (gradient by workgroup: 256 lanes, 512 from 1024 CH columns on, 1024 from 4096 CH on: at 6000 bf16 columns 110, 147 and 210 us, at 24000 115, 110 and 115, at 50000 140, 133 and 125)
 template <typename T, int CH>
 void launch_grad(const Rows& g, const GradIn& in, hipStream_t stream) {
-	const dim3 grid = rows_grid(g);
 	if constexpr (CH == 1) {
-		logp_grad_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, in);
+		logp_grad_team_kernel<T, CH, 16><<<team_grid<16>(g), dim3(256), 0, stream>>>(g, in);
 	} else {
-		const int threads = row_threads(g, CH);
-		if (threads == 64) logp_grad_kernel<T, CH, 64><<<grid, dim3(64), 0, stream>>>(g, in);
-		else if (threads == 256) logp_grad_kernel<T, CH, 256><<<grid, dim3(256), 0, stream>>>(g, in);
-		else logp_grad_kernel<T, CH, 1024><<<grid, dim3(1024), 0, stream>>>(g, in);
+		if (g.V <= 64 * CH) logp_grad_team_kernel<T, CH, 16><<<team_grid<16>(g), dim3(256), 0, stream>>>(g, in);
+		else if (by_team<CH>(g, true)) logp_grad_team_kernel<T, CH, 64><<<team_grid<64>(g), dim3(256), 0, stream>>>(g, in);
+		else if (g.V < 1024 * CH) logp_grad_kernel<T, CH, 256><<<rows_grid(g), dim3(256), 0, stream>>>(g, in);
+		else if (g.V < 4096 * CH) logp_grad_kernel<T, CH, 512><<<rows_grid(g), dim3(512), 0, stream>>>(g, in);
+		else logp_grad_kernel<T, CH, 1024><<<rows_grid(g), dim3(1024), 0, stream>>>(g, in);
 	}
 }
 template <typename T, int CH>
 void launch_policy(const Rows& g, const Policy& p, hipStream_t stream) {
 	const dim3 grid = rows_grid(g);
-	NOVIC_ROW_SHAPES(g.V, (policy_kernel<T, CH, TH, NC><<<grid, dim3(TH), 0, stream>>>(g, p)),
-	                 (policy_long_kernel<T, CH, TH><<<grid, dim3(TH), 0, stream>>>(g, p)))
+	if constexpr (CH == 1) {
+		policy_team_kernel<T, CH, 16, 1><<<team_grid<16>(g), dim3(256), 0, stream>>>(g, p);
+	} else if (by_team<CH>(g, true)) {
+		NOVIC_TEAM_SHAPES(g.V, 4, (policy_team_kernel<T, CH, L, NC><<<team_grid<L>(g), dim3(256), 0, stream>>>(g, p)))
+	} else {
+		NOVIC_ROW_SHAPES(g.V, (policy_kernel<T, CH, TH, NC><<<grid, dim3(TH), 0, stream>>>(g, p)), (policy_long_kernel<T, CH, TH><<<grid, dim3(TH), 0, stream>>>(g, p)))
+	}
 }
 #define NOVIC_ROW_TYPES(type, V, FN, ...)                                             \
 	if (V < 8) NOVIC_TYPE_SWITCH(type, T, (FN<T, 1>(__VA_ARGS__)))                       \
@@ -881,22 +1035,20 @@ extern "C" int novic_token_logprobs_bwd(const void* logits, int type, int64_t ld
 	return 0;
 }
 
-// Pair by pair where the pairs alone fill the chip (two workgroups of eight waves a unit) and a wave's registers hold a row; else row by row, with a launch over the pairs between
-// the two over the rows.
+// Pair by pair where the pairs alone fill the chip (two workgroups of eight waves a unit), a wave's registers hold a row and the row is long enough for a wave; else row by row, with
+// the pairs between the two launches over the rows.
 constexpr int FUSED_PAIRS = 512;
-bool pair_by_pair(const Rows& g, int type) { return g.A / 2 >= FUSED_PAIRS && 2 * g.T <= PAIR_ROWS && g.V <= PAIR_VECTORS * 64 * (type == NOVIC_TYPE_F32 ? 4 : 8); }
+bool pair_by_pair(const Rows& g, int type) {
+	const int ch = type == NOVIC_TYPE_F32 ? 4 : 8;
+	return g.A / 2 >= FUSED_PAIRS && 2 * g.T <= PAIR_ROWS && g.V > 64 * ch && g.V <= PAIR_VECTORS * 64 * ch;
+}
 template <typename T, int CH>
 void launch_pairs(const Rows& g, const LogpOut& o, const Pref& q, hipStream_t stream) {
 	const dim3 grid((unsigned)q.n), block(PAIR_WAVES * 64);
-	if constexpr (CH == 1) {
-		pref_pair_kernel<T, CH, 1><<<grid, block, 0, stream>>>(g, o, q);
-	} else {
-		if (g.V <= 64 * CH) pref_pair_kernel<T, CH, 1><<<grid, block, 0, stream>>>(g, o, q);
-		else if (g.V <= 4 * 64 * CH) pref_pair_kernel<T, CH, 4><<<grid, block, 0, stream>>>(g, o, q);
-		else if (g.V <= 8 * 64 * CH) pref_pair_kernel<T, CH, 8><<<grid, block, 0, stream>>>(g, o, q);
-		else if (g.V <= 12 * 64 * CH) pref_pair_kernel<T, CH, 12><<<grid, block, 0, stream>>>(g, o, q);
-		else pref_pair_kernel<T, CH, PAIR_VECTORS><<<grid, block, 0, stream>>>(g, o, q);
-	}
+	if (g.V <= 4 * 64 * CH) pref_pair_kernel<T, CH, 4><<<grid, block, 0, stream>>>(g, o, q);
+	else if (g.V <= 8 * 64 * CH) pref_pair_kernel<T, CH, 8><<<grid, block, 0, stream>>>(g, o, q);
+	else if (g.V <= 12 * 64 * CH) pref_pair_kernel<T, CH, 12><<<grid, block, 0, stream>>>(g, o, q);
+	else pref_pair_kernel<T, CH, PAIR_VECTORS><<<grid, block, 0, stream>>>(g, o, q);
 }
 
 // workspace: diff [2n T] fp64, each [2][n] fp64, norm [2n T] float2, coef [2n], total fp64, scale
@@ -931,12 +1083,20 @@ extern "C" int novic_preference_loss(const void* logits, int type, int64_t ldl, 
 	const Pref q = {diff, weight, n, T, kind, beta, smoothing, grad_scale, margin, coef, each, total, (float*)w, stats};
 	if (pair_by_pair(g, type)) {
 		if (weight) pref_weight_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q);
-		NOVIC_ROW_TYPES(type, V, launch_pairs, g, o, q, stream)
+		if (type == NOVIC_TYPE_F32) launch_pairs<float, 4>(g, o, q, stream);
+		else if (type == NOVIC_TYPE_BF16) launch_pairs<bf16, 8>(g, o, q, stream);
+		else launch_pairs<f16, 8>(g, o, q, stream);
 		pref_finish_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q);
 	} else {
 		o.diff = diff;
 		NOVIC_ROW_TYPES(type, V, launch_logp, g, o, stream)
-		pref_all_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q, lanes_for(T));
+		const int lanes = lanes_for(T);
+		if ((long long)n * lanes <= 2048) {  // two rounds of one workgroup: shorter than a second launch
+			pref_all_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q, lanes);
+		} else {
+			pref_each_kernel<<<dim3((unsigned)(((long long)n * lanes + 255) / 256)), dim3(256), 0, stream>>>(q, lanes);
+			pref_finish_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q);
+		}
 		if (dlogits) {
 			GradIn in = {};
 			in.norm = norm; in.grad = coef; in.lda = 1; in.ldt = 0; in.scale = q.scale;

@@ -305,12 +305,18 @@ def test_dropout_beyond_32_bits():
 class Tokens:
 	"""Logits in a wider buffer, targets, a padding mask with rows that leave a sequence empty, NaN logits where a position does not count."""
 
-	def __init__(self, A, T, V, dtype, extra=0, shift=0, seed=0, tok=torch.int64, scale=3.0, empty=True):
+	def __init__(self, A, T, V, dtype, extra=0, shift=0, seed=0, tok=torch.int64, scale=3.0, empty=True, offsets=False):
 		g = gen(seed + A * 31 + T * 7 + V)
 		self.A, self.T, self.V, self.dtype, self.g = A, T, V, dtype, g
 		self.box = Box(A * T, V, dtype, extra, shift, normal(g, A * T, V, scale=scale))
 		self.logits = self.box.t
-		self.target = torch.randint(0, V, (A, T), generator=g, device=DEV).to(tok)
+		if offsets:  # rows of negative numbers, rows of positive ones, rows of zeros of both signs, rows with most of the vocabulary masked out
+			kind = torch.arange(A * T, device=DEV) % 5
+			self.logits += torch.tensor([0.0, -60.0, 40.0, 0.0, 0.0], device=DEV)[kind].to(dtype)[:, None]
+			self.logits[kind == 3] *= 0.0
+			self.logits[3::5] = torch.where(torch.rand(self.logits[3::5].shape, generator=g, device=DEV) < 0.5, -0.0, 0.0).to(dtype)
+			self.logits[4::5, 3:] = float("-inf")
+		self.target = torch.randint(0, 3 if offsets else V, (A, T), generator=g, device=DEV).to(tok)
 		length = torch.randint(1, T + 1, (A,), generator=g, device=DEV)
 		if empty and A > 2:
 			length[1] = 0
@@ -325,7 +331,8 @@ class Tokens:
 		self.lse = torch.logsumexp(x, 1)
 		self.p = (x - self.lse[:, None]).exp()
 		self.onehot = torch.zeros_like(x).scatter_(1, at, 1.0)
-		self.d = (x - x.max(1, keepdim=True).values).abs()  # distance from the maximum: an exponential is off by that many u, relative
+		self.d = (x - x.max(1, keepdim=True).values).abs().nan_to_num(posinf=0.0)  # (of a masked element: its exponential is a zero)
+		# distance from the maximum: an exponential is off by that many u, relative
 		self.lp = ((x.gather(1, at).squeeze(1) - self.lse).view(A, T) * self.valid).detach()
 		# log s: K u for the sum, 4 u + the mean distance for the exponentials
 		self.dlp = (U * (K + 4 + (self.p * self.d).sum(1).view(A, T)) + U * self.lp.abs()) * self.valid
@@ -437,7 +444,8 @@ PREF = [("sigmoid", 0.0, 0.1), ("sigmoid", 0.2, 0.5), ("hinge", 0.0, 0.3), ("squ
 
 @pytest.mark.parametrize("kind,e,beta", PREF)
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("n,T,V,extra,shift", [(1, 1, 5, 0, 0), (1, 1, 97, 3, 1), (3, 7, 257, 0, 0), (40, 7, 1000, 24, 0), (2, 130, 6912, 0, 0), (5, 12, 6911, 1, 0), (2, 4, 40001, 0, 0), (1, 3, 70001, 7, 0), (1500, 2, 33, 0, 0)])
+@pytest.mark.parametrize("n,T,V,extra,shift", [(520, 7, 1000, 24, 0), (513, 3, 2500, 3, 1), (512, 12, 6912, 0, 0), (515, 2, 8191, 0, 0), (512, 32, 300, 0, 0), (512, 33, 300, 0, 0), (600, 2, 8200, 0, 0), (512, 5, 4097, 0, 0),
+                                               (700, 40, 17, 0, 0), (1, 1, 5, 0, 0), (1, 1, 97, 3, 1), (3, 7, 257, 0, 0), (40, 7, 1000, 24, 0), (2, 130, 6912, 0, 0), (5, 12, 6911, 1, 0), (2, 4, 40001, 0, 0), (1, 3, 70001, 7, 0), (1500, 2, 33, 0, 0)])
 def test_preference(n, T, V, extra, shift, dtype, kind, e, beta):
 	s = Tokens(2 * n, T, V, dtype, extra, shift, tok=torch.int32 if n == 3 else torch.int64)
 	ref = (s.lp + 0.7 * torch.randn(2 * n, T, generator=s.g, device=DEV, dtype=torch.double)).float()
@@ -475,6 +483,51 @@ def test_preference(n, T, V, extra, shift, dtype, kind, e, beta):
 	assert torch.equal(only, stats)
 	call(stats=only, dlogits=s.logits)  # in place
 	assert torch.equal(s.logits, dl.t) and torch.equal(only, stats)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("op", ["logprob", "preference", "policy"])
+@pytest.mark.parametrize("n,T,V", [(3000, 2, 17), (3000, 2, 100), (700, 5, 700), (520, 6, 1500), (600, 4, 3000), (520, 4, 6000), (30, 4, 6000), (20, 3, 9000), (4, 2, 70000)])
+def test_rows_of_all_kinds(n, T, V, op, dtype):
+	"""Rows whose numbers are all negative, all positive, zeros of both signs, or mostly masked out: gradients by every form of the kernels, at row counts that choose each."""
+	A = 2 * n
+	s = Tokens(A, T, V, dtype, offsets=True)
+	old = torch.where(s.valid, s.lp - 0.1, 0.0).float()
+	d = Box(A * T, V, dtype, 5, 1)
+	adv = normal(s.g, A)
+	if op == "logprob":
+		lse, out = torch.empty(A * T, device=DEV), torch.empty(A, T, device=DEV)
+		ops.token_logprobs(s.logits, s.target, out, pad=s.pad, lse=lse)
+		near(out, s.lp, s.dlp, "logp")
+		ops.token_logprobs_bwd(s.logits, s.target, lse, adv, d.t, pad=s.pad)
+		coef = adv.double()[:, None].expand(A, T)
+		dcoef = torch.zeros_like(coef)
+		want = s.dlogits(coef)
+		# lse rounds where it is kept, up to 70 here
+		bound = s.dlogits_bound(coef, dcoef, want, dtype) + (coef.abs() * s.valid).reshape(-1, 1) * s.p * (U * (3 * s.lse.abs().view(-1, 1) + s.d) + s.dlp.view(-1, 1))
+	elif op == "preference":
+		stats = torch.empty(3, device=DEV)
+		ops.preference_loss(s.logits, s.target, old, stats, beta=0.3, pad=s.pad, dlogits=d.t, grad_scale=float(n))
+		u = torch.where(s.valid, s.lp - old.double(), 0.0).sum(1)
+		z = 0.3 * (u[:n] - u[n:])
+		c = -0.3 * torch.sigmoid(-z)
+		coef = torch.cat([c, -c])[:, None].expand(A, T)
+		dz = 0.3 * (s.dlp.sum(1)[:n] + s.dlp.sum(1)[n:])
+		dcoef = torch.cat([dz, dz])[:, None].expand(A, T) * 0.3 * 0.25 + 8 * U * coef.abs()
+		want = s.dlogits(coef)
+		bound = s.dlogits_bound(coef, dcoef, want, dtype)
+		near(stats[0], -torch.nn.functional.logsigmoid(z).mean(), float(dz.mean()) + 4 * U)
+	else:
+		stats = torch.empty(4, device=DEV)
+		count = float(s.valid.sum())
+		ops.policy_loss(s.logits, s.target, old, adv, stats, pad=s.pad, dlogits=d.t, grad_scale=count)
+		q = torch.where(s.valid, (s.lp - old.double()).exp(), 0.0)  # 1.105: inside the clip range
+		coef = -q * adv.double()[:, None]
+		dcoef = coef.abs() * (s.dlp + 16 * U)
+		want = s.dlogits(coef)
+		bound = s.dlogits_bound(coef, dcoef, want, dtype)
+	near(d.t, want, bound, f"dlogits of {op}")
+	assert d.intact()
 
 
 def test_preference_without_weight_or_tokens():
