@@ -4,8 +4,10 @@
 //   backward   g = dy gamma, xhat = (x - mu) rstd:  dx = dx_in + rstd (g - mean(g) - xhat mean(g xhat));  dgamma = sum_rows dy xhat, dbeta = sum_rows dy
 //
 // HBM-bound both ways: each element is read once and written once, the row lives in registers between its statistics and its output (the two-pass variance costs no second
-// read), statistics and sums in fp32.  A row belongs to a team of 16, 64 or 256 lanes, the
-// smallest that holds it in at most four vectors a lane, or of 512, whose lanes take up to eight (with 1024 lanes a lane has 128 registers, and the backward pass spills).
+// read), statistics and sums in fp32.  A row belongs to a team of 16, 64 or 256 lanes, the smallest that holds it in about four vectors a lane, or of 512, whose lanes take up to
+// eight (with 1024 lanes a lane has 128 registers: 5 % faster backward at 16384 columns, but one type's form spills, and 6 to 40 % slower forward).  What is read once is loaded, and
+// gradients are stored, past the caches.  MI355X: forward [57344 x 512] fp32 -> bf16 30.4 us (5.8 TB/s), [65792 x 1280] bf16 66 us (5.1); backward [65792 x 1280] bf16 with both
+// affine gradients and the residual's added 121 us (5.6 TB/s, of it 7 us in the reduction of the partial rows; without those hints 132).
 #include "novic_hip.h"
 #include "rowvec.hpp"
 
@@ -31,8 +33,10 @@ __device__ __forceinline__ void team_sum2(float& a, float& b, float* scratch, in
 	}
 }
 
+// waves a SIMD: what the grid of plan() counts on
+constexpr int fwd_waves(int lanes, int held) { return held <= 24 && (lanes <= 256 || held <= 16) ? 4 : lanes <= 256 ? 3 : 2; }
 template <typename XT, typename YT, int CH, int LANES, int NC>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_fwd_kernel(const XT* x, long long ldx, const float* __restrict__ gamma,
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256, fwd_waves(LANES, NC * CH)) void layernorm_stats_fwd_kernel(const XT* x, long long ldx, const float* __restrict__ gamma,
                                                                                        const float* __restrict__ beta, YT* y, long long ldy,
                                                                                        float* __restrict__ mean_out, float* __restrict__ rstd_out, int rows, int E, float eps) {
 	constexpr int THREADS = LANES > 256 ? LANES : 256, TEAMS = THREADS / LANES;
@@ -61,29 +65,32 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_fwd
 	for (int row0 = first; row0 < rows; row0 += stride) {
 		const int row = LANES < 64 ? row0 : __builtin_amdgcn_readfirstlane(row0);
 		load(next, min(row0 + stride, rows - 1));  // requested before this row is reduced
-		float v[NC][CH], s = 0.f, q = 0.f, off = 0.f, none = 0.f;
+		float s = 0.f, q = 0.f, off = 0.f, none = 0.f;
 #pragma unroll
-		for (int c = 0; c < NC; ++c)
+		for (int c = 0; c < NC; ++c) {
 #pragma unroll
-			for (int i = 0; i < CH; ++i) {
-				v[c][i] = raw[c].get(i);
-				if (c < NC - 1 || es[c] + i >= (c * LANES + lane) * CH) s += v[c][i];
-			}
+			for (int i = 0; i < CH; ++i)
+				if (c < NC - 1 || es[c] + i >= (c * LANES + lane) * CH) s += raw[c].get(i);
+			if constexpr (NC * CH > 16) forget(raw[c]);  // (the deviations of a long row are formed where they are used: held, they would cost the registers of a resident workgroup)
+		}
 		team_sum2<LANES>(s, none, scratch, turn);
 		// The first mean is off by the sum's rounding, which a row far from zero would carry into every element: the deviations' own mean `off` corrects it, at no extra reduction.
 		float mean = s / (float)E;
 #pragma unroll
-		for (int c = 0; c < NC; ++c)
+		for (int c = 0; c < NC; ++c) {
 #pragma unroll
 			for (int i = 0; i < CH; ++i) {
-				v[c][i] -= mean;
+				const float d = raw[c].get(i) - mean;
 				if (c < NC - 1 || es[c] + i >= (c * LANES + lane) * CH) {
-					q += v[c][i] * v[c][i];
-					off += v[c][i];
+					q += d * d;
+					off += d;
 				}
 			}
+			if constexpr (NC * CH > 16) forget(raw[c]);
+		}
 		team_sum2<LANES>(q, off, scratch, turn);
 		off *= inv;
+		const float first_mean = mean;
 		mean += off;
 		const float var = q * inv - off * off;
 		const float rstd = rsqrtf((var < 0.f ? 0.f : var) + eps);  // (a NaN stays one)
@@ -97,7 +104,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_fwd
 			float o[CH];
 #pragma unroll
 			for (int i = 0; i < CH; ++i) {
-				float t = (v[c][i] - off) * rstd * gm[c].get(i);
+				float t = ((raw[c].get(i) - first_mean) - off) * rstd * gm[c].get(i);
 				if (beta) t += bt[c].get(i);
 				o[i] = t;
 			}
@@ -263,21 +270,25 @@ __global__ __launch_bounds__(1024) void layernorm_stats_reduce_kernel(const floa
 	}
 }
 
-#ifndef DIRECT
-#define DIRECT 4
-#endif
 struct Plan {
 	int lanes, chunks, blocks;
 };
 // ch: elements of a lane's vector
 Plan plan(int rows, int E, int ch, bool bwd) {
 	Plan p;
-	p.lanes = E <= 16 * ch ? 16 : E <= 256 * ch ? 64 : E <= 1024 * ch ? 256 : 512;
+	// Forward: sixteen lanes up to four vectors each ([200000 x 100] fp32 -> bf16: 25 us, by wave 60), a wave up to five fp32 vectors ([65792 x 1280]: 95 us, with 256 lanes 129; more would spill).
+	// Backward: sixteen lanes up to 256 columns (the same rows: 49 and 86 us; at 512 bf16 columns 51 and 39), a wave up to four vectors a lane.
+	const int narrow = bwd ? 256 : 64 * ch, wide = ch == 4 && !bwd ? 1280 : 256 * ch;
+	p.lanes = E <= narrow ? 16 : E <= wide ? 64 : E <= 1024 * ch ? 256 : 512;
 	p.chunks = (E + p.lanes * ch - 1) / (p.lanes * ch);
 	const int teams = p.lanes > 256 ? 1 : 256 / p.lanes;
-	// Forward: four workgroups a unit (1024: 30.2 us, 2048: 31.8, 4096: 30.9 on [57344 x 512] fp32 -> bf16).  Backward: as many as are resident at once, two a unit, one of 512
-	// lanes: each leaves a partial row of both gradients behind.  A handful of rows is one workgroup's business, which needs no second launch.
-	const int most = !bwd ? 1024 : p.lanes > 256 ? 256 : rows <= DIRECT * teams ? 1 : 512;
+	// Forward: as many workgroups as are resident at once, up to four a unit (more are slower: 1024 of them 30.2 us, 2048 31.8 on [57344 x 512]; a part of them left over for a second
+	// round is worse).  Backward: as many as are resident, two a unit or one: each leaves a partial row of both gradients behind.  A handful of rows is one workgroup's business,
+	// which needs no second launch (16 rows of 512: 9.4 us a call, with it 13.5).
+	const int held = p.chunks * ch;
+	int most;
+	if (bwd) most = rows <= 4 * teams ? 1 : p.lanes > 256 && held > 16 ? 256 : 512;
+	else most = p.lanes > 256 ? (held <= 16 ? 512 : 256) : held <= 24 ? 1024 : 768;
 	p.blocks = (int)std::min<long long>(most, ((long long)rows + teams - 1) / teams);
 	return p;
 }
@@ -285,11 +296,11 @@ int chunk_elems(int x_type, int y_type, int E) { return E < 8 ? 1 : (x_type != N
 
 // (a shape that no width of this vector length asks for is not compiled)
 #define NOVIC_LN_CASE(LANES, NC, CALL)                                                         \
-	if constexpr ((NC - 1) * LANES * CH < 16384 && (CH > 1 || LANES == 16)) {                    \
+	if constexpr ((NC - 1) * LANES * CH < 16384 && (CH > 1 || (LANES == 16 && NC == 1))) {                    \
 		if (p.lanes == LANES && p.chunks == NC) { constexpr int L = LANES, N = NC; CALL; }          \
 	}
 #define NOVIC_LN_SHAPES(CALL)                                                                                                                             \
-	NOVIC_LN_CASE(16, 1, CALL)                                                                                                                            \
+	NOVIC_LN_CASE(16, 1, CALL) NOVIC_LN_CASE(16, 2, CALL) NOVIC_LN_CASE(16, 3, CALL) NOVIC_LN_CASE(16, 4, CALL)                                           \
 	NOVIC_LN_CASE(64, 1, CALL) NOVIC_LN_CASE(64, 2, CALL) NOVIC_LN_CASE(64, 3, CALL) NOVIC_LN_CASE(64, 4, CALL)                                           \
 	NOVIC_LN_CASE(256, 2, CALL) NOVIC_LN_CASE(256, 3, CALL) NOVIC_LN_CASE(256, 4, CALL)                                                                    \
 	NOVIC_LN_CASE(512, 3, CALL) NOVIC_LN_CASE(512, 4, CALL) NOVIC_LN_CASE(512, 5, CALL) NOVIC_LN_CASE(512, 6, CALL) NOVIC_LN_CASE(512, 7, CALL) NOVIC_LN_CASE(512, 8, CALL)
@@ -301,8 +312,9 @@ bool types_ok(int x_type, int y_type) {
 template <typename XT, typename YT, int CH>
 void launch_fwd(const Plan& p, const void* x, long long ldx, const float* gamma, const float* beta, void* y, long long ldy, float* mean, float* rstd, int rows, int E, float eps,
                 hipStream_t stream) {
-	NOVIC_LN_SHAPES((layernorm_stats_fwd_kernel<XT, YT, CH, L, N><<<dim3(p.blocks), dim3(L > 256 ? L : 256), 0, stream>>>((const XT*)x, ldx, gamma, beta, (YT*)y, ldy,
-	                                    mean, rstd, rows, E, eps)))
+#define NOVIC_LN_FWD (layernorm_stats_fwd_kernel<XT, YT, CH, L, N><<<dim3(p.blocks), dim3(L > 256 ? L : 256), 0, stream>>>((const XT*)x, ldx, gamma, beta, (YT*)y, ldy, mean, rstd, rows, E, eps))
+	NOVIC_LN_SHAPES(NOVIC_LN_FWD)
+	if constexpr (CH == 4) { NOVIC_LN_CASE(64, 5, NOVIC_LN_FWD) }
 }
 template <typename XT, typename YT, int CH>
 void launch_bwd(const Plan& p, const void* dy, long long lddy, const void* x, long long ldx, const float* gamma, const float* mean, const float* rstd, const void* dx_in, long long ldi,

@@ -194,6 +194,8 @@ struct RowStream {
 	__device__ __forceinline__ static void grad(const T* row, T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
 		RawVec<T, CH> raw[UNROLL], next[UNROLL];
 		load(raw, row, 0, V, lane);
+		// xt may come through the scalar cache, whose loads are not ordered with vector stores: it has to be here before the first of them, where out is row
+		asm volatile("" : "+v"(xt));
 		for (int e = 0; e < V; e += UNROLL * LANES * CH) {
 			if (e + UNROLL * LANES * CH < V) load(next, row, e + UNROLL * LANES * CH, V, lane);  // (before this piece's stores, also where out is row: no vector is in both)
 #pragma unroll
@@ -283,6 +285,7 @@ struct TeamRow {
 		s = team_sum<LANES>(t);
 	}
 	__device__ __forceinline__ void grad(T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
+		asm volatile("" : "+v"(xt));  // (as in RowStream)
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
 			if (!any(c, V)) continue;
@@ -473,7 +476,7 @@ struct Pref {
 	float* margin;        // [n] or null
 	float* coef;          // [2 n]: gradient of sum_i w_i l_i to a sequence's u
 	double* each;         // [2][n]: w l, w z
-	double* total;        // device scalar: sum(w)
+	double* total;        // device scalar: sum(w), or null
 	float* scale;         // device scalar: grad_scale / sum(w)
 	float* stats;         // [3]: loss, mean margin, sum(w)
 };
@@ -628,10 +631,10 @@ __global__ __launch_bounds__(1024) void pref_finish_kernel(const Pref g) {
 // A pair by one workgroup, loss and gradient.  The pair's rows (at most 64) are lanes' business first: each wave asks for all targets and reference values and knows the rows that
 // count from a ballot.  Those are dealt to the waves in turn; the row that a wave sums last stays in its registers up to its gradient, any others are read again (a pair's
 // time later: out of L2 or the memory-side cache).  Sixteen vectors a lane are what 128 registers hold beside the rest of the kernel.
-constexpr int PAIR_WAVES = 8, PAIR_ROWS = 64, PAIR_VECTORS = 16;
+constexpr int PAIR_WAVES = 8, PAIR_ROWS = 64, PAIR_VECTORS = 16, PAIR_WEIGHTS = 4096;
 template <typename T, int CH, int NC>
 __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Rows g, const LogpOut o, const Pref q) {
-	__shared__ double part[2][PAIR_WAVES];
+	__shared__ double part[3][PAIR_WAVES];
 	const int i = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, rows = 2 * q.T;
 	const int my_half = lane >= q.T, my_a = my_half ? q.n + i : i, my_t = lane - my_half * q.T;  // lane k stands for row k: the preferred sequence's, then the other's
 	int my_target = -1;
@@ -639,6 +642,16 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 	if (lane < rows) {
 		my_target = counted_target(g, my_a, my_t);
 		my_ref = o.ref[my_a * o.ldref + my_t];
+	}
+	double total = 0.0;  // of the weights: few enough are added up by every workgroup (q.total is null), which saves a launch in front of this one
+	if (q.weight && !q.total) {
+		float w[PAIR_WEIGHTS / (PAIR_WAVES * 64)];
+#pragma unroll
+		for (int k = 0; k < PAIR_WEIGHTS / (PAIR_WAVES * 64); ++k) w[k] = q.weight[min(k * PAIR_WAVES * 64 + (int)threadIdx.x, q.n - 1)];
+#pragma unroll
+		for (int k = 0; k < PAIR_WEIGHTS / (PAIR_WAVES * 64); ++k) total += k * PAIR_WAVES * 64 + (int)threadIdx.x < q.n ? (double)w[k] : 0.0;
+#pragma unroll
+		for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
 	}
 	const unsigned long long counted = __ballot(my_target >= 0), others = __ballot(lane < rows && my_target < 0);
 	const int have = __popcll(counted), none = __popcll(others);
@@ -668,6 +681,7 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 	if (lane == 0) {
 		part[0][wave] = u[0];
 		part[1][wave] = u[1];
+		part[2][wave] = total;
 	}
 	for (int l = PAIR_WAVES - 1 - wave; l < none; l += PAIR_WAVES) {
 		const int kz = nth(others, l), rz = row_of(kz);
@@ -675,16 +689,19 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 		if (lane == 0) put_logp(o, rz, kz >= q.T ? q.n + i : i, kz >= q.T ? kz - q.T : kz, false, 0.0, 0.f, 1.f);
 	}
 	__syncthreads();
-	u[0] = u[1] = 0.0;
+	u[0] = u[1] = total = 0.0;
 #pragma unroll
 	for (int w = 0; w < PAIR_WAVES; ++w) {
 		u[0] += part[0][w];
 		u[1] += part[1][w];
+		total += part[2][w];
 	}
+	if (!q.weight) total = (double)q.n;
+	else if (q.total) total = *q.total;
 	const double z = pref_margin(q, u[0], u[1]);
 	if (threadIdx.x == PAIR_WAVES * 64 - 1) pref_terms(q, i, z);  // (the last wave: it has the fewest rows)
 	if (!g.dlogits) return;
-	const float c = pref_slope(q, i, z) * pref_scale(q, q.weight ? *q.total : (double)q.n);
+	const float c = pref_slope(q, i, z) * pref_scale(q, total);
 	if (wave >= have) return;
 	float coef = k >= q.T ? -c : c;
 	tile.grad((T*)g.dlogits + (long long)r * g.ldd, g.V, lane, target, xt, M, -coef / s, coef);
@@ -700,6 +717,7 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 }
 
 // ---- policy loss -------------------------------------------------------------------------------------------------------------------------------------------------
+constexpr int COUNT_HERE = 1024;
 struct Policy {
 	const float *old, *adv, *ref;  // old, ref [A][T]; adv at adv[a * lda + t * ldt]
 	long long ldold, ldref, lda, ldt;
@@ -710,8 +728,8 @@ struct Policy {
 	int* len;          // [A]: counted rows of a sequence
 	int* part;         // [2][parts]: counted rows, sequences with any, of the sequences of one block of policy_count_kernel
 	int parts;
-	float4* each;      // [A T]: loss, KL, clipped, each times the row's share of the mean
-	double* slices;    // [64][3]: sums over the slices of policy_finish_kernel
+	float4* each;      // [A T]: loss, KL, clipped, each times the row's share of the mean; whether it counts
+	double* slices;    // [64][4]: sums over the slices of policy_finish_kernel
 	float* stats;      // [4]: loss, mean KL, clipped share, counted rows
 };
 __global__ __launch_bounds__(256) void policy_count_kernel(const Rows g, const Policy p, int lanes) {
@@ -740,13 +758,51 @@ __global__ __launch_bounds__(256) void policy_count_kernel(const Rows g, const P
 	__syncthreads();
 	if (threadIdx.x < 2) p.part[threadIdx.x * p.parts + blockIdx.x] = red[4 * threadIdx.x] + red[4 * threadIdx.x + 1] + red[4 * threadIdx.x + 2] + red[4 * threadIdx.x + 3];
 }
-// the counts of all blocks, by one wave (at most 64 parts)
-__device__ __forceinline__ int policy_total(const Policy& p, int which) {
-	const int lane = threadIdx.x & 63;
-	int n = lane < p.parts ? p.part[which * p.parts + lane] : 0;
+// The counts that a row's share of the mean needs: from policy_count_kernel, or, for at most COUNT_HERE rows (parts = 0), taken by every workgroup for itself, which saves the launch.
+struct Counts {
+	int total;             // counted rows, or (per_seq) sequences that have any
+	const uint8_t* flags;  // LDS: a flag a row, or null
+};
+__device__ __forceinline__ Counts policy_counts(const Rows& g, const Policy& p, uint8_t* flags, int* red) {
+	Counts c = {0, nullptr};
+	if (p.parts > 0) {  // the counts of all blocks, by each wave (at most 64 parts)
+		const int lane = threadIdx.x & 63;
+		c.total = lane < p.parts ? p.part[(p.per_seq ? p.parts : 0) + lane] : 0;
+#pragma unroll
+		for (int o = 32; o > 0; o >>= 1) c.total += __shfl_xor(c.total, o, 64);
+		return c;
+	}
+	const int R = g.A * g.T;
+	for (int r = threadIdx.x; r < R; r += blockDim.x) flags[r] = counted_target(g, r / g.T, r % g.T) >= 0;
+	__syncthreads();
+	int n = 0;
+	for (int r = threadIdx.x; r < R; r += blockDim.x) {
+		bool yes = flags[r];
+		if (p.per_seq && yes)  // the sequence's first counted row stands for it
+			for (int k = r - 1; yes && k >= r - r % g.T; --k) yes = !flags[k];
+		n += yes;
+	}
 #pragma unroll
 	for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-	return n;
+	if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
+	__syncthreads();
+	for (int w = 0; w < (int)(blockDim.x >> 6); ++w) c.total += red[w];
+	c.flags = flags;
+	return c;
+}
+// a row's share of the mean, by a team of LANES lanes
+template <int LANES>
+__device__ __forceinline__ float policy_share(const Rows& g, const Policy& p, const Counts& c, int a, int lane) {
+	if (!p.per_seq) return 1.f / (float)c.total;
+	int n = 0;
+	if (c.flags) {
+		for (int t = lane; t < g.T; t += LANES) n += c.flags[a * g.T + t];
+#pragma unroll
+		for (int o = LANES / 2; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+	} else {
+		n = p.len[a];
+	}
+	return 1.f / ((float)n * (float)c.total);
 }
 // The gradient of the whole loss to a row's log-probability.  The ratio and the KL term are exponentials of small differences that were formed in fp64.
 struct PolicyRow {
@@ -767,15 +823,12 @@ __device__ __forceinline__ float policy_grad(const Policy& p, int a, int t, doub
 	}
 	return g * share * p.grad_scale;
 }
-__device__ __forceinline__ float policy_share(const Rows& g, const Policy& p, int a) {
-	return p.per_seq ? 1.f / ((float)p.len[a] * (float)policy_total(p, 1)) : 1.f / (float)policy_total(p, 0);
-}
 // what one thread of the row writes: its log-probability and its terms of the means
 __device__ __forceinline__ void policy_put(const Rows& g, const Policy& p, int r, int a, int t, double lp, float share, const PolicyRow& w) {
 	const double kl = p.ref ? expm1(w.d) - w.d : 0.0;
 	if (p.logp) p.logp[a * p.ldo + t] = (float)lp;
 	const double l = (w.whole ? -(double)w.q * w.adv : -(double)w.held * w.adv) + (double)p.kl_coef * kl;
-	p.each[r] = make_float4((float)(l * share), (float)(kl * share), w.whole ? 0.f : share, 0.f);
+	p.each[r] = make_float4((float)(l * share), (float)(kl * share), w.whole ? 0.f : share, 1.f);
 }
 __device__ __forceinline__ void policy_put_none(const Rows& g, const Policy& p, int r, int a, int t) {
 	if (p.logp) p.logp[a * p.ldo + t] = 0.f;
@@ -784,6 +837,8 @@ __device__ __forceinline__ void policy_put_none(const Rows& g, const Policy& p, 
 template <typename T, int CH, int THREADS, int NC>
 __global__ __launch_bounds__(THREADS) void policy_kernel(const Rows g, const Policy p) {
 	__shared__ float red[2 * THREADS / 64];
+	__shared__ uint8_t flags[COUNT_HERE];
+	__shared__ int counts[THREADS / 64];
 	const int r = row_index(g);
 	if (r < 0) return;
 	const int a = r / g.T, t = r - a * g.T;
@@ -797,7 +852,7 @@ __global__ __launch_bounds__(THREADS) void policy_kernel(const Rows g, const Pol
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
 	RowTile<T, CH, THREADS, NC> tile;
 	tile.load(row, g.V);
-	const float xt = (float)row[target], share = policy_share(g, p, a);
+	const float xt = (float)row[target], share = policy_share<64>(g, p, policy_counts(g, p, flags, counts), a, threadIdx.x & 63);
 	tile.sum(g.V, red);
 	const double lp = row_logp(xt, tile.M, tile.s);
 	PolicyRow w;
@@ -808,6 +863,8 @@ __global__ __launch_bounds__(THREADS) void policy_kernel(const Rows g, const Pol
 template <typename T, int CH, int THREADS>
 __global__ __launch_bounds__(THREADS) void policy_long_kernel(const Rows g, const Policy p) {
 	__shared__ float red[2 * THREADS / 64];
+	__shared__ uint8_t flags[COUNT_HERE];
+	__shared__ int counts[THREADS / 64];
 	const int r = row_index(g);
 	if (r < 0) return;
 	const int a = r / g.T, t = r - a * g.T;
@@ -819,7 +876,7 @@ __global__ __launch_bounds__(THREADS) void policy_long_kernel(const Rows g, cons
 		return;
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
-	const float xt = (float)row[target], share = policy_share(g, p, a);
+	const float xt = (float)row[target], share = policy_share<64>(g, p, policy_counts(g, p, flags, counts), a, threadIdx.x & 63);
 	float M, s;
 	block_row_sum<T, CH, THREADS>(row, g.V, red, M, s);
 	const double lp = row_logp(xt, M, s);
@@ -833,7 +890,9 @@ __global__ __launch_bounds__(256) void policy_team_kernel(const Rows g, const Po
 	const int lane = threadIdx.x % LANES;
 	TeamRow<T, CH, LANES, NC> tile;
 	Walk<LANES> now(g);
-	const int total = policy_total(p, p.per_seq ? 1 : 0);
+	__shared__ uint8_t flags[COUNT_HERE];
+	__shared__ int four[4];
+	const Counts shared = policy_counts(g, p, flags, four);
 	while (!now.done(g)) {
 		const int target = now.target(g);
 		const bool counts = target >= 0;
@@ -843,7 +902,7 @@ __global__ __launch_bounds__(256) void policy_team_kernel(const Rows g, const Po
 		if (counts) {
 			tile.load(row, g.V, lane);
 			xt = (float)row[target];
-			share = p.per_seq ? 1.f / ((float)p.len[now.a] * (float)total) : 1.f / (float)total;
+			share = policy_share<LANES>(g, p, shared, now.a, lane);
 		}
 		const Walk<LANES> next = now.next(g);
 		if (counts) {
@@ -865,7 +924,7 @@ __global__ __launch_bounds__(256) void policy_team_kernel(const Rows g, const Po
 __global__ __launch_bounds__(1024) void policy_finish_kernel(const Rows g, const Policy p) {
 	__shared__ double red[48];
 	const long long R = (long long)g.A * g.T, slice = (R + gridDim.x - 1) / gridDim.x, first = blockIdx.x * slice, end = min(first + slice, R);
-	double l = 0.0, k = 0.0, c = 0.0;
+	double l = 0.0, k = 0.0, c = 0.0, n = 0.0;
 	for (long long r0 = first + threadIdx.x; r0 < end; r0 += 8 * 1024) {  // eight rows a thread requested at once
 		float4 v[8];
 #pragma unroll
@@ -876,35 +935,28 @@ __global__ __launch_bounds__(1024) void policy_finish_kernel(const Rows g, const
 			l += (double)v[i].x;
 			k += (double)v[i].y;
 			c += (double)v[i].z;
+			n += (double)v[i].w;
 		}
 	}
 	sum3_1024(l, k, c, red);
-	const int n = gridDim.x == 1 ? policy_total(p, 0) : 0;
+	__syncthreads();
+	double none = 0.0, zero = 0.0;
+	sum3_1024(n, none, zero, red);
 	if (threadIdx.x == 0) {
-		if (gridDim.x == 1) {
-			p.stats[0] = (float)l;
-			p.stats[1] = (float)k;
-			p.stats[2] = (float)c;
-			p.stats[3] = (float)n;
-		} else {
-			p.slices[3 * blockIdx.x] = l;
-			p.slices[3 * blockIdx.x + 1] = k;
-			p.slices[3 * blockIdx.x + 2] = c;
+		const double v[4] = {l, k, c, n};
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			if (gridDim.x == 1) p.stats[i] = (float)v[i];
+			else p.slices[4 * blockIdx.x + i] = v[i];
 		}
 	}
 }
-__global__ __launch_bounds__(64) void policy_slices_kernel(const Policy p) {
-	const int lane = threadIdx.x;
-	double v[3];
+__global__ __launch_bounds__(256) void policy_slices_kernel(const Policy p) {
+	const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+	double v = p.slices[4 * lane + w];
 #pragma unroll
-	for (int i = 0; i < 3; ++i) {
-		v[i] = p.slices[3 * lane + i];
-#pragma unroll
-		for (int o = 32; o > 0; o >>= 1) v[i] += __shfl_xor(v[i], o, 64);
-	}
-	const int n = policy_total(p, 0);
-	if (lane < 3) p.stats[lane] = (float)(lane == 0 ? v[0] : lane == 1 ? v[1] : v[2]);
-	if (lane == 3) p.stats[3] = (float)n;
+	for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+	if (lane == 0) p.stats[w] = (float)v;
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------------------------------------
@@ -916,10 +968,12 @@ __global__ __launch_bounds__(64) void policy_slices_kernel(const Policy p) {
 	else if (V <= 4096 * CH) { constexpr int TH = 1024, NC = 4; REG; }                                       \
 	else if (V <= 8192 * CH) { constexpr int TH = 1024, NC = 8; REG; }                                       \
 	else { constexpr int TH = 1024; LONG; }
-// Rows by team: sixteen lanes up to 64 CH columns, a wave with up to MOST vectors a lane beyond
+constexpr int SHORT = 128;
+// Rows by team: sixteen lanes up to SHORT CH columns (600 bf16 columns: 73 us, by wave 159), a wave with up to MOST vectors a lane beyond
 #define NOVIC_TEAM_SHAPES(V, MOST, CALL)                                                                   \
 	if (V <= 16 * CH) { constexpr int L = 16, NC = 1; CALL; }                                                \
 	else if (V <= 64 * CH) { constexpr int L = 16, NC = 4; CALL; }                                           \
+	else if (V <= SHORT * CH) { constexpr int L = 16, NC = SHORT / 16; CALL; }                               \
 	else if (MOST == 4 || V <= 4 * 64 * CH) { constexpr int L = 64, NC = 4; CALL; }                          \
 	else if (V <= 8 * 64 * CH) { constexpr int L = 64, NC = MOST < 8 ? MOST : 8; CALL; }                     \
 	else { constexpr int L = 64, NC = MOST; CALL; }
@@ -951,7 +1005,7 @@ void launch_grad(const Rows& g, const GradIn& in, hipStream_t stream) {
 	if constexpr (CH == 1) {
 		logp_grad_team_kernel<T, CH, 16><<<team_grid<16>(g), dim3(256), 0, stream>>>(g, in);
 	} else {
-		if (g.V <= 64 * CH) logp_grad_team_kernel<T, CH, 16><<<team_grid<16>(g), dim3(256), 0, stream>>>(g, in);
+		if (g.V <= SHORT * CH) logp_grad_team_kernel<T, CH, 16><<<team_grid<16>(g), dim3(256), 0, stream>>>(g, in);
 		else if (by_team<CH>(g, true)) logp_grad_team_kernel<T, CH, 64><<<team_grid<64>(g), dim3(256), 0, stream>>>(g, in);
 		else if (g.V < 1024 * CH) logp_grad_kernel<T, CH, 256><<<rows_grid(g), dim3(256), 0, stream>>>(g, in);
 		else if (g.V < 4096 * CH) logp_grad_kernel<T, CH, 512><<<rows_grid(g), dim3(512), 0, stream>>>(g, in);
@@ -1080,9 +1134,10 @@ extern "C" int novic_preference_loss(const void* logits, int type, int64_t ldl, 
 	double* total = (double*)w; w += 16;
 	LogpOut o = {};
 	o.logp = logp; o.ldo = ldo; o.ref = ref; o.ldref = ldref; o.norm = dlogits ? norm : nullptr;
-	const Pref q = {diff, weight, n, T, kind, beta, smoothing, grad_scale, margin, coef, each, total, (float*)w, stats};
+	Pref q = {diff, weight, n, T, kind, beta, smoothing, grad_scale, margin, coef, each, total, (float*)w, stats};
 	if (pair_by_pair(g, type)) {
-		if (weight) pref_weight_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q);
+		if (weight && n > PAIR_WEIGHTS) pref_weight_kernel<<<dim3(1), dim3(1024), 0, stream>>>(q);
+		else q.total = nullptr;
 		if (type == NOVIC_TYPE_F32) launch_pairs<float, 4>(g, o, q, stream);
 		else if (type == NOVIC_TYPE_BF16) launch_pairs<bf16, 8>(g, o, q, stream);
 		else launch_pairs<f16, 8>(g, o, q, stream);
@@ -1107,10 +1162,10 @@ extern "C" int novic_preference_loss(const void* logits, int type, int64_t ldl, 
 	return 0;
 }
 
-// workspace: len [A], part [2][64], slices [64][3] fp64, each [A T] float4
+// workspace: len [A], part [2][64], slices [64][4] fp64, each [A T] float4
 extern "C" uint64_t novic_policy_loss_ws(int A, int T) {
 	if (A <= 0 || T <= 0) return 0;
-	return up16(4ull * A) + up16(8 * COUNT_PARTS) + 24 * SLICES + 16ull * A * T;
+	return up16(4ull * A) + up16(8 * COUNT_PARTS) + 32 * SLICES + 16ull * A * T;
 }
 extern "C" int novic_policy_loss(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int A, int T, int V,
                                  const float* old_logp, int64_t ldold, const float* adv, int64_t adv_lda, int64_t adv_ldt, const float* ref, int64_t ldref, float clip_lo, float clip_hi,
@@ -1136,16 +1191,17 @@ extern "C" int novic_policy_loss(const void* logits, int type, int64_t ldl, cons
 	char* w = (char*)ws;
 	p.len = (int*)w; w += up16(4ull * A);
 	p.part = (int*)w; w += up16(8 * COUNT_PARTS);
-	p.slices = (double*)w; w += 24 * SLICES;
+	p.slices = (double*)w; w += 32 * SLICES;
 	p.each = (float4*)w;
-	p.parts = count_parts(A, T);
+	const bool counted = (long long)A * T > COUNT_HERE;
+	p.parts = counted ? count_parts(A, T) : 0;
 	p.stats = stats;
-	policy_count_kernel<<<dim3(p.parts), dim3(256), 0, stream>>>(g, p, lanes_for(T));
+	if (counted) policy_count_kernel<<<dim3(p.parts), dim3(256), 0, stream>>>(g, p, lanes_for(T));
 	NOVIC_ROW_TYPES(type, V, launch_policy, g, p, stream)
 	// one workgroup reads its rows' terms at some 50 GB/s: beyond 8192 rows (a batch of loads a thread) 64 of them and one launch more are shorter
 	const bool sliced = (long long)A * T > 8192;
 	policy_finish_kernel<<<dim3(sliced ? SLICES : 1), dim3(1024), 0, stream>>>(g, p);
-	if (sliced) policy_slices_kernel<<<dim3(1), dim3(64), 0, stream>>>(p);
+	if (sliced) policy_slices_kernel<<<dim3(1), dim3(256), 0, stream>>>(p);
 	NOVIC_LAUNCH_CHECK();
 	return 0;
 }

@@ -530,6 +530,23 @@ def test_rows_of_all_kinds(n, T, V, op, dtype):
 	assert d.intact()
 
 
+@pytest.mark.parametrize("dtype,n,T,V", [(F32, 512, 12, 6912), (BF16, 600, 3, 9000), (F16, 40, 20, 40000), (BF16, 600, 4, 3000), (F32, 600, 4, 200)])
+def test_gradients_in_place_every_time(dtype, n, T, V):
+	"""The gradient written over its logits has the bits of the one written beside them, twenty times over: the target's logit is read before anything may be stored there."""
+	s = Tokens(2 * n, T, V, dtype)
+	old, adv = s.lp.float(), normal(s.g, 2 * n)
+	keep, d = s.logits.clone(), torch.empty(2 * n * T, V, device=DEV, dtype=dtype)
+	st, st4, lse = torch.empty(3, device=DEV), torch.empty(4, device=DEV), (s.lse * s.valid.view(-1)).float()
+	for call in (lambda o: ops.preference_loss(s.logits, s.target, old, st, beta=0.2, pad=s.pad, dlogits=o), lambda o: ops.policy_loss(s.logits, s.target, old, adv, st4, pad=s.pad, dlogits=o),
+	             lambda o: ops.token_logprobs_bwd(s.logits, s.target, lse, adv, o, pad=s.pad)):
+		call(d)
+		for _ in range(20):
+			s.logits.copy_(keep)
+			call(s.logits)
+			assert torch.equal(s.logits, d)
+		s.logits.copy_(keep)
+
+
 def test_preference_without_weight_or_tokens():
 	s = Tokens(6, 4, 50, BF16)
 	ref, stats, d = torch.zeros(6, 4, device=DEV), torch.full((3,), 7.0, device=DEV), torch.full((24, 50), 7.0, device=DEV, dtype=BF16)
