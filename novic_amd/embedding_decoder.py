@@ -1176,6 +1176,71 @@ class PrefixedIterDecoder(EmbeddingDecoder):
 		self._run_backward(sv, self.flat_grad())
 		return stats
 
+	# ---- fine-tuning on the decoder's own candidates (the reference trains with cross entropy only): log-probabilities of given labels, preferences between two labels of an
+	# embedding, clipped policy steps on sampled labels.  Gradients are ACCUMULATED into the flat gradient buffer, as by forward_backward; the optimizer step is the caller's. ----
+	def token_logprobs(self, embed, target, target_padding) -> torch.Tensor:
+		"""fp32 log-probabilities of the target tokens, target's shape, 0 where target_padding says so: what a frozen decoder contributes as ref_logprobs and a sampling one as
+		old_logprobs.  target: [B][C], or [2][B][C] for the two labels of each preference (no dropout, whatever the mode)."""
+		flat, pad, rep = self._finetune_inputs(target, target_padding)
+		out = torch.empty(flat.shape, dtype=torch.float32, device=flat.device)
+		if not out.numel():
+			return out.view(target.shape)
+		sv = self._run_forward(embed, flat, pad, None, rep, rep > 1, only_pred=False, train=False, drop=Dropout(0.0, 0, 0), tag="fwd")
+		ops.token_logprobs(self._buf(sv, "logits")[:, :self.target_config.vocab_size], flat, out, pad=pad)
+		return out.view(target.shape)
+
+	def forward_backward_preference(self, embed, target, target_padding, ref_logprobs, *, beta: float = 0.1, kind: str = "sigmoid", smoothing: float = 0.0, weight=None,
+	                                loss_scale: float = 1.0, tag: str = "train"):
+		"""Forward + backward of a preference step: label target[0][b] of embedding b is preferred to target[1][b] (target, target_padding, ref_logprobs [2][B][C]; ops.preference_loss
+		says what kind, smoothing and weight [B] do).  Returns (stats [loss, mean margin, sum of weights], margins [B], log-probabilities [2][B][C])."""
+		if target.ndim != 3 or target.shape[0] != 2:
+			raise ValueError(f"a preference step takes targets [2][B][C], got {tuple(target.shape)}")
+		flat, pad, rep = self._finetune_inputs(target, target_padding)
+		if ref_logprobs.shape != target.shape:
+			raise ValueError(f"ref_logprobs {tuple(ref_logprobs.shape)} for a target of {tuple(target.shape)}")
+		stats, margin, logp = (torch.empty(shape, dtype=torch.float32, device=target.device) for shape in ((3,), (target.shape[1],), flat.shape))
+		ref = ref_logprobs.reshape(flat.shape)
+		self._finetune_step(embed, flat, pad, rep, tag, lambda logits: ops.preference_loss(logits, flat, ref, stats, beta=beta, kind=kind, smoothing=smoothing, pad=pad,
+		                                                                                      weight=weight, logp=logp, margin=margin, dlogits=logits, grad_scale=loss_scale))
+		return stats, margin, logp.view(target.shape)
+
+	def forward_backward_policy(self, embed, target, target_padding, old_logprobs, advantage, *, clip=(0.2, 0.2), ref_logprobs=None, kl_coef: float = 0.0, per_sequence: bool = False,
+	                            loss_scale: float = 1.0, tag: str = "train"):
+		"""Forward + backward of a clipped policy step on sampled labels target [B][C] with their log-probabilities at sampling time and an advantage each ([B], or [B][C]); the other
+		arguments as ops.policy_loss.  Returns (stats [loss, KL, clipped share, counted tokens], log-probabilities [B][C])."""
+		if target.ndim != 2:
+			raise ValueError(f"a policy step takes targets [B][C], got {tuple(target.shape)}")
+		flat, pad, rep = self._finetune_inputs(target, target_padding)
+		stats, logp = (torch.empty(shape, dtype=torch.float32, device=target.device) for shape in ((4,), flat.shape))
+		self._finetune_step(embed, flat, pad, rep, tag, lambda logits: ops.policy_loss(logits, flat, old_logprobs, advantage, stats, clip=clip, ref=ref_logprobs, kl_coef=kl_coef,
+		                                                                                  per_sequence=per_sequence, pad=pad, logp=logp, dlogits=logits, grad_scale=loss_scale))
+		return stats, logp
+
+	@staticmethod
+	def _finetune_inputs(target, target_padding):
+		"""(sequences [A][C], their padding, labels per embedding): [2][B][C] lists the embeddings' first labels, then their second ones.  A label's log-probability is that of its own
+		tokens: num_end_loss > 1 (end tokens that the cross entropy counts on top) has no part in it."""
+		if target_padding is not None and target_padding.shape != target.shape:
+			raise ValueError(f"target_padding {tuple(target_padding.shape)} for a target of {tuple(target.shape)}")
+		if target.ndim not in (2, 3):
+			raise ValueError(f"targets are [B][C] or [labels][B][C], got {tuple(target.shape)}")
+		C = target.shape[-1]
+		rows = target.numel() // C if C else 0
+		return target.reshape(rows, C).contiguous(), None if target_padding is None else target_padding.reshape(rows, C).contiguous(), target.shape[0] if target.ndim == 3 else 1
+
+	def _finetune_step(self, embed, flat, pad, rep, tag, loss):
+		"""Forward pass that keeps its activations (every position: the losses add up over sequences), loss(logits) writing the gradient over the logits, backward pass.  The storage
+		columns behind the vocabulary are exact zeros before and after."""
+		if not flat.numel():
+			raise ValueError("a fine-tuning step takes at least one token")
+		drop = self.next_dropout()
+		if self.training:
+			sv = self._run_forward(embed, flat, pad, None, rep, rep > 1, only_pred=False, train=True, drop=drop, tag=tag)
+		else:
+			sv = self._run_forward_eval_keep(embed, flat, pad, None, rep, rep > 1, drop, tag)
+		loss(self._buf(sv, "logits")[:, :self.target_config.vocab_size])
+		self._run_backward(sv, self.flat_grad())
+
 	def _run_forward_eval_keep(self, embed, target, target_padding, target_weight, mrep, multi_first, drop, tag, compact: bool = False):
 		"""Forward that keeps activations (for backward) but with every dropout off (model.eval() training, used by parity tests)."""
 		saved = (self.input_dropout, self.layer_dropout)
