@@ -17,10 +17,26 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 // A row's sums are seen from M = fl(m log2 e), m its maximum: an exponential is one fma and one v_exp_f32, exp2(x LOG2E - M), and M's rounding takes part in nothing but the choice
-// of the point, m' = M / LOG2E, from which x - m' is measured (in fp64, once a row).
-__device__ __forceinline__ float expo(float x, float M) { return __builtin_amdgcn_exp2f(fmaf(x, LOG2E, -M)); }
-__device__ __forceinline__ float point(float m) { return m * LOG2E; }
-__device__ __forceinline__ double from_point(float M) { return (double)M / (double)LOG2E; }
+// of the point, m' = M / LOG2E, from which x - m' is measured (in fp64, once a row).  Beyond FAR (a row that is masked with -1e30 or its type's lowest value throughout) that rounding
+// would be 64 and more, and the product need not be a number.  Two numbers there are equal or differ by 128 at least, so that powers of two tell them apart as well as
+// exponentials do: m is the point itself.
+constexpr float FAR = 1.4e9f;
+struct Point {
+	float M, L;
+};
+__device__ __forceinline__ Point point(float m) {
+	const bool far = fabsf(m) > FAR;
+	return {far ? m : m * LOG2E, far ? 1.f : LOG2E};
+}
+__device__ __forceinline__ float expo(float x, Point p) { return __builtin_amdgcn_exp2f(fmaf(x, p.L, -p.M)); }
+__device__ __forceinline__ double from_point(float m) {  // m'
+	return fabsf(m) > FAR ? (double)m : (double)(m * LOG2E) * (1.0 / (double)LOG2E);
+}
+// what a sum seen from the point of `from` is multiplied by to be seen from that of `to`
+__device__ __forceinline__ float shift(float from, float to) {
+	const Point a = point(from), b = point(to);
+	return a.L == b.L ? __builtin_amdgcn_exp2f(a.M - b.M) : 0.f;
+}
 
 struct Rows {
 	const void* logits;
@@ -45,7 +61,7 @@ __device__ __forceinline__ int row_index(const Rows& g) {
 	return r < (long long)g.A * g.T ? (int)r : -1;
 }
 
-// log(s) to 1e-16 relative of a sum in [1, 2^31] without the cost of a double-precision logarithm: s = 2^k f, f in [0.7, 1.42): |logf(f)| < 0.36, its rounding 3e-8 absolute
+// log(s) to 1e-16 relative of a sum (up to 2^64 V) without the cost of a double-precision logarithm: s = 2^k f, f in [0.7, 1.42): |logf(f)| < 0.36, its rounding 3e-8 absolute
 __device__ __forceinline__ double log_wide(float s) {
 	int k;
 	float f = frexpf(s, &k);
@@ -85,7 +101,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 template <typename T, int CH, int THREADS, int NC>
 struct RowTile {
 	float x[NC][CH];
-	float M, s;
+	float m, s;
 	__device__ __forceinline__ static int own(int c) { return (c * THREADS + (int)threadIdx.x) * CH; }
 	__device__ __forceinline__ static int at(int c, int V) { return min(own(c), V - CH); }
 	__device__ __forceinline__ void load(const T* row, int V) {
@@ -104,7 +120,8 @@ struct RowTile {
 		for (int c = 0; c < NC; ++c)
 #pragma unroll
 			for (int i = 0; i < CH; ++i) t = fmaxf(t, x[c][i]);
-		M = point(block_max<THREADS>(t, red));
+		m = block_max<THREADS>(t, red);
+		const Point at_m = point(m);
 		t = 0.f;
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
@@ -115,7 +132,7 @@ struct RowTile {
 			}
 #pragma unroll
 			for (int i = 0; i < CH; ++i) {
-				x[c][i] = expo(x[c][i], M);
+				x[c][i] = expo(x[c][i], at_m);
 				if ((c + 1) * THREADS * CH > V && at(c, V) + i < own(c)) x[c][i] = 0.f;
 				t += x[c][i];
 			}
@@ -150,9 +167,9 @@ struct RowStream {
 			for (int u = 0; u < UNROLL; ++u) raw[u] = load_vec<T, CH>(elem(row, min(e + (u * LANES + lane) * CH, V - CH)));
 		}
 	}
-	// point and sum over this lane's part, with a running maximum; the next vectors are requested before the present ones are added
-	__device__ __forceinline__ static void sum(const T* row, int V, int lane, float& tM, float& ts) {
-		tM = -INFINITY;
+	// maximum and sum over this lane's part; the next vectors are requested before the present ones are added
+	__device__ __forceinline__ static void sum(const T* row, int V, int lane, float& tm, float& ts) {
+		tm = -INFINITY;
 		ts = 0.f;
 		RawVec<T, CH> raw[UNROLL], next[UNROLL];
 		load(raw, row, 0, V, lane);
@@ -165,33 +182,32 @@ struct RowStream {
 				for (int i = 0; i < CH; ++i) top = fmaxf(top, raw[u].get(i));
 				forget(raw[u]);  // (else its elements stay unpacked from one use to the next, at twice the registers)
 			}
-			const float M = fmaxf(tM, point(top)), base = M == -INFINITY ? 0.f : M;  // (nothing but -inf yet: their exponentials are zeros)
-			ts *= __builtin_amdgcn_exp2f(tM - base);
+			const float m = fmaxf(tm, top), base = m == -INFINITY ? 0.f : m;  // (nothing but -inf yet: their exponentials are zeros)
+			const Point at_m = point(base);
+			ts *= shift(tm, base);
 			if (e + UNROLL * LANES * CH <= V) {
 #pragma unroll
 				for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-					for (int i = 0; i < CH; ++i) ts += expo(raw[u].get(i), base);
+					for (int i = 0; i < CH; ++i) ts += expo(raw[u].get(i), at_m);
 			} else {
 #pragma unroll
 				for (int u = 0; u < UNROLL; ++u) {
 					const int e0 = e + (u * LANES + lane) * CH, es = min(e0, V - CH);
 #pragma unroll
-					for (int i = 0; i < CH; ++i) ts += es + i >= e0 ? expo(raw[u].get(i), base) : 0.f;
+					for (int i = 0; i < CH; ++i) ts += es + i >= e0 ? expo(raw[u].get(i), at_m) : 0.f;
 				}
 			}
-			tM = M;
+			tm = m;
 #pragma unroll
 			for (int u = 0; u < UNROLL; ++u) raw[u] = next[u];
 		}
 	}
 	// a lane's sum seen from the row's point
-	__device__ __forceinline__ static float scaled(float tM, float ts, float M) {
-		const float base = M == -INFINITY ? 0.f : M;
-		return ts * __builtin_amdgcn_exp2f((tM == -INFINITY ? base : tM) - base);
-	}
-	// out = k exp2(x log2 e - M), and coef more at the target (whose logit is xt); out may be row
-	__device__ __forceinline__ static void grad(const T* row, T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
+	__device__ __forceinline__ static float scaled(float tm, float ts, float m) { return ts * shift(tm, m == -INFINITY ? 0.f : m); }
+	// out = k exp(x - m), and coef more at the target (whose logit is xt); out may be row
+	__device__ __forceinline__ static void grad(const T* row, T* out, int V, int lane, int target, float xt, float m, float k, float coef) {
+		const Point at_m = point(m);
 		RawVec<T, CH> raw[UNROLL], next[UNROLL];
 		load(raw, row, 0, V, lane);
 		// xt may come through the scalar cache, whose loads are not ordered with vector stores: it has to be here before the first of them, where out is row
@@ -202,7 +218,7 @@ struct RowStream {
 			for (int u = 0; u < UNROLL; ++u) {
 				float o[CH];
 #pragma unroll
-				for (int i = 0; i < CH; ++i) o[i] = k * expo(raw[u].get(i), M);
+				for (int i = 0; i < CH; ++i) o[i] = k * expo(raw[u].get(i), at_m);
 				if (e + UNROLL * LANES * CH <= V) {
 					store_vec<true>(elem(out + (e + u * LANES * CH), lane * CH), o);
 				} else {
@@ -213,7 +229,7 @@ struct RowStream {
 #pragma unroll
 			for (int u = 0; u < UNROLL; ++u) raw[u] = next[u];
 		}
-		if ((target / CH) % LANES == lane) out[target] = (T)(k * expo(xt, M) + coef);
+		if ((target / CH) % LANES == lane) out[target] = (T)(k * expo(xt, at_m) + coef);
 	}
 	__device__ __forceinline__ static void zero(T* row, int V, int lane) {
 		float o[CH];
@@ -268,23 +284,27 @@ struct TeamRow {
 		}
 		return team_max<LANES>(t);
 	}
-	__device__ __forceinline__ void sum(int V, int lane, float& M, float& s) {
-		M = point(top());
+	// (where the team is a wave the point goes to scalar registers)
+	__device__ __forceinline__ static Point at_max(float m) { return point(LANES == 64 ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(m))) : m); }
+	__device__ __forceinline__ void sum(int V, int lane, float& m, float& s) {
+		m = top();
+		const Point at_m = at_max(m);
 		float t = 0.f;
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
 			forget(raw[c]);  // (else its elements stay unpacked from one use to the next, at twice the registers)
 			if (whole(c, V)) {
 #pragma unroll
-				for (int i = 0; i < CH; ++i) t += expo(raw[c].get(i), M);
+				for (int i = 0; i < CH; ++i) t += expo(raw[c].get(i), at_m);
 			} else if (any(c, V)) {
 #pragma unroll
-				for (int i = 0; i < CH; ++i) t += at(V, lane) + i >= cut(c, V, lane) ? expo(raw[c].get(i), M) : 0.f;
+				for (int i = 0; i < CH; ++i) t += at(V, lane) + i >= cut(c, V, lane) ? expo(raw[c].get(i), at_m) : 0.f;
 			}
 		}
 		s = team_sum<LANES>(t);
 	}
-	__device__ __forceinline__ void grad(T* out, int V, int lane, int target, float xt, float M, float k, float coef) {
+	__device__ __forceinline__ void grad(T* out, int V, int lane, int target, float xt, float m, float k, float coef) {
+		const Point at_m = at_max(m);
 		asm volatile("" : "+v"(xt));  // (as in RowStream)
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
@@ -292,7 +312,7 @@ struct TeamRow {
 			forget(raw[c]);
 			float o[CH];
 #pragma unroll
-			for (int i = 0; i < CH; ++i) o[i] = k * expo(raw[c].get(i), M);
+			for (int i = 0; i < CH; ++i) o[i] = k * expo(raw[c].get(i), at_m);
 			if (whole(c, V)) {
 				store_vec<true>(elem(out + base(c, V), at(V, lane)), o);
 			} else if (at(V, lane) >= cut(c, V, lane)) {
@@ -303,7 +323,7 @@ struct TeamRow {
 					if (at(V, lane) + i >= cut(c, V, lane) && cut(c, V, lane) < V) *elem(out + base(c, V), at(V, lane) + i) = (T)o[i];
 			}
 		}
-		if (owner(target, V) == lane) out[target] = (T)(k * expo(xt, M) + coef);
+		if (owner(target, V) == lane) out[target] = (T)(k * expo(xt, at_m) + coef);
 	}
 	// the lane that stores element v (after which it may store it once more)
 	__device__ __forceinline__ static int owner(int v, int V) {
@@ -346,25 +366,25 @@ struct LogpOut {
 	float* lse;        // [A T] or null: the row's log-sum-exp
 	const float* ref;  // [A][T] or null
 	double* diff;      // [A T] or null: lp - ref, 0 where the row does not count
-	float2* norm;      // [A T] or null: (M, 1 / s)
+	float2* norm;      // [A T] or null: (m, 1 / s)
 	long long ldo, ldref;
 };
 __device__ __forceinline__ float reference(const LogpOut& o, int a, int t) { return o.diff ? o.ref[a * o.ldref + t] : 0.f; }
-__device__ __forceinline__ void put_logp(const LogpOut& o, int r, int a, int t, bool counts, double lp, float M, float s, float ref = 0.f) {
+__device__ __forceinline__ void put_logp(const LogpOut& o, int r, int a, int t, bool counts, double lp, float m, float s, float ref = 0.f) {
 	if (o.logp) o.logp[a * o.ldo + t] = counts ? (float)lp : 0.f;
-	if (o.lse) o.lse[r] = counts ? (float)(from_point(M) + log_wide(s)) : 0.f;
+	if (o.lse) o.lse[r] = counts ? (float)(from_point(m) + log_wide(s)) : 0.f;
 	if (o.diff) o.diff[r] = counts ? lp - (double)ref : 0.0;
-	if (o.norm) o.norm[r] = counts ? make_float2(M, 1.f / s) : make_float2(0.f, 0.f);
+	if (o.norm) o.norm[r] = counts ? make_float2(m, 1.f / s) : make_float2(0.f, 0.f);
 }
 
 template <typename T, int CH, int THREADS>
-__device__ __forceinline__ void block_row_sum(const T* row, int V, float* red, float& M, float& s) {
-	float tM, ts;
-	RowStream<T, CH, THREADS>::sum(row, V, threadIdx.x, tM, ts);
-	M = block_max<THREADS>(tM, red);
-	s = block_sum<THREADS>(RowStream<T, CH, THREADS>::scaled(tM, ts, M), red + THREADS / 64);
+__device__ __forceinline__ void block_row_sum(const T* row, int V, float* red, float& m, float& s) {
+	float tm, ts;
+	RowStream<T, CH, THREADS>::sum(row, V, threadIdx.x, tm, ts);
+	m = block_max<THREADS>(tm, red);
+	s = block_sum<THREADS>(RowStream<T, CH, THREADS>::scaled(tm, ts, m), red + THREADS / 64);
 }
-__device__ __forceinline__ double row_logp(float xt, float M, float s) { return ((double)xt - from_point(M)) - log_wide(s); }
+__device__ __forceinline__ double row_logp(float xt, float m, float s) { return ((double)xt - from_point(m)) - log_wide(s); }
 template <typename T, int CH, int THREADS>
 __global__ __launch_bounds__(THREADS) void logp_kernel(const Rows g, const LogpOut o) {
 	__shared__ float red[2 * THREADS / 64];
@@ -378,9 +398,9 @@ __global__ __launch_bounds__(THREADS) void logp_kernel(const Rows g, const LogpO
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
 	const float xt = (float)row[target], ref = reference(o, a, t);
-	float M, s;
-	block_row_sum<T, CH, THREADS>(row, g.V, red, M, s);
-	if (threadIdx.x == 0) put_logp(o, r, a, t, true, row_logp(xt, M, s), M, s, ref);
+	float m, s;
+	block_row_sum<T, CH, THREADS>(row, g.V, red, m, s);
+	if (threadIdx.x == 0) put_logp(o, r, a, t, true, row_logp(xt, m, s), m, s, ref);
 }
 
 template <typename T, int CH, int LANES, int NC>
@@ -398,9 +418,9 @@ __global__ __launch_bounds__(256) void logp_team_kernel(const Rows g, const Logp
 			ref = reference(o, now.a, now.t);
 		}
 		const Walk<LANES> next = now.next(g);
-		float M = 0.f, s = 1.f;
-		if (target >= 0) tile.sum(g.V, lane, M, s);
-		if (lane == 0) put_logp(o, now.r, now.a, now.t, target >= 0, target >= 0 ? row_logp(xt, M, s) : 0.0, M, s, ref);
+		float m = 0.f, s = 1.f;
+		if (target >= 0) tile.sum(g.V, lane, m, s);
+		if (lane == 0) put_logp(o, now.r, now.a, now.t, target >= 0, target >= 0 ? row_logp(xt, m, s) : 0.0, m, s, ref);
 		now = next;
 	}
 }
@@ -408,24 +428,24 @@ __global__ __launch_bounds__(256) void logp_team_kernel(const Rows g, const Logp
 // ---- gradient of log-probabilities: dlogits = coef (1[v = target] - exp(x - m) / s) ----------------------------------------------------------------------------------
 struct GradIn {
 	const float* lse;     // [A T], or null:
-	const float2* norm;   // [A T] (M, 1 / s)
+	const float2* norm;   // [A T] (m, 1 / s)
 	const float* grad;    // element (a, t) at grad[a * lda + t * ldt]
 	long long lda, ldt;
 	const float* scale;   // device scalar or null
 };
-// dlogits = k exp2(x log2 e - M) + (coef at the target)
-__device__ __forceinline__ void grad_terms(const GradIn& in, int r, int a, int t, float& M, float& k, float& coef) {
+// dlogits = k exp(x - m) + (coef at the target)
+__device__ __forceinline__ void grad_terms(const GradIn& in, int r, int a, int t, float& m, float& k, float& coef) {
 	coef = in.grad[a * in.lda + t * in.ldt];
 	if (in.scale) coef *= *in.scale;
 	k = -coef;
 	if (in.norm) {
 		const float2 n = in.norm[r];
-		M = n.x;
+		m = n.x;
 		k *= n.y;
 	} else {
-		const float lse = in.lse[r];
-		M = point(lse);
-		k *= __builtin_amdgcn_exp2f(-fmaf(lse, LOG2E, -M));  // (what the point's rounding took: s is what lse says, seen from M)
+		m = in.lse[r];
+		const Point at_m = point(m);
+		k *= __builtin_amdgcn_exp2f(-fmaf(m, at_m.L, -at_m.M));  // (what the point's rounding took: s is what lse says, seen from M)
 	}
 }
 template <typename T, int CH, int THREADS>
@@ -440,10 +460,10 @@ __global__ __launch_bounds__(THREADS) void logp_grad_kernel(const Rows g, const 
 		return;
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
-	float M, k, coef;
-	grad_terms(in, r, a, t, M, k, coef);
+	float m, k, coef;
+	grad_terms(in, r, a, t, m, k, coef);
 	const float xt = (float)row[target];  // (used by the lane that owns the target alone, which loads it before it writes there: out may be row)
-	RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, M, k, coef);
+	RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, m, k, coef);
 }
 
 template <typename T, int CH, int LANES>
@@ -458,10 +478,10 @@ __global__ __launch_bounds__(256) void logp_grad_team_kernel(const Rows g, const
 		if (target < 0) {
 			Stream::zero(out, g.V, lane);
 		} else {
-			float M, k, coef;
-			grad_terms(in, now.r, now.a, now.t, M, k, coef);
+			float m, k, coef;
+			grad_terms(in, now.r, now.a, now.t, m, k, coef);
 			const T* row = (const T*)g.logits + (long long)now.r * g.ldl;
-			Stream::grad(row, out, g.V, lane, target, (float)row[target], M, k, coef);
+			Stream::grad(row, out, g.V, lane, target, (float)row[target], m, k, coef);
 		}
 		now = next;
 	}
@@ -661,22 +681,22 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 	auto row_of = [&](int k) { return (k >= q.T ? q.n + i : i) * q.T + (k >= q.T ? k - q.T : k); };
 	auto of_lane = [&](int v, int k) { return __builtin_amdgcn_readlane(v, k); };
 	double u[2] = {0.0, 0.0};
-	auto counted_row = [&](int k, int r, float xt, float M, float s) {  // lane 0: the row's log-probability, added to its sequence
-		const double lp = row_logp(xt, M, s), d = lp - (double)__int_as_float(of_lane(__float_as_int(my_ref), k));
+	auto counted_row = [&](int k, int r, float xt, float m, float s) {  // lane 0: the row's log-probability, added to its sequence
+		const double lp = row_logp(xt, m, s), d = lp - (double)__int_as_float(of_lane(__float_as_int(my_ref), k));
 		u[0] += k >= q.T ? 0.0 : d;
 		u[1] += k >= q.T ? d : 0.0;
-		if (lane == 0) put_logp(o, r, k >= q.T ? q.n + i : i, k >= q.T ? k - q.T : k, true, lp, M, s);
+		if (lane == 0) put_logp(o, r, k >= q.T ? q.n + i : i, k >= q.T ? k - q.T : k, true, lp, m, s);
 	};
 	TeamRow<T, CH, 64, NC> tile;
-	float M = 0.f, s = 1.f, xt = 0.f;
+	float m = 0.f, s = 1.f, xt = 0.f;
 	int k = 0, r = 0, target = 0;
 	for (int l = wave + (have - 1 - wave) / PAIR_WAVES * PAIR_WAVES; wave < have && l >= 0; l -= PAIR_WAVES) {
 		k = nth(counted, l), r = row_of(k), target = of_lane(my_target, k);
 		const T* row = (const T*)g.logits + (long long)r * g.ldl;
 		tile.load(row, g.V, lane);
 		xt = (float)row[target];
-		tile.sum(g.V, lane, M, s);
-		counted_row(k, r, xt, M, s);
+		tile.sum(g.V, lane, m, s);
+		counted_row(k, r, xt, m, s);
 	}
 	if (lane == 0) {
 		part[0][wave] = u[0];
@@ -704,7 +724,7 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 	const float c = pref_slope(q, i, z) * pref_scale(q, total);
 	if (wave >= have) return;
 	float coef = k >= q.T ? -c : c;
-	tile.grad((T*)g.dlogits + (long long)r * g.ldd, g.V, lane, target, xt, M, -coef / s, coef);
+	tile.grad((T*)g.dlogits + (long long)r * g.ldd, g.V, lane, target, xt, m, -coef / s, coef);
 	for (int l = wave + PAIR_WAVES; l < have; l += PAIR_WAVES) {
 		k = nth(counted, l), r = row_of(k), target = of_lane(my_target, k);
 		const T* row = (const T*)g.logits + (long long)r * g.ldl;
@@ -854,11 +874,11 @@ __global__ __launch_bounds__(THREADS) void policy_kernel(const Rows g, const Pol
 	tile.load(row, g.V);
 	const float xt = (float)row[target], share = policy_share<64>(g, p, policy_counts(g, p, flags, counts), a, threadIdx.x & 63);
 	tile.sum(g.V, red);
-	const double lp = row_logp(xt, tile.M, tile.s);
+	const double lp = row_logp(xt, tile.m, tile.s);
 	PolicyRow w;
 	const float coef = policy_grad(p, a, t, lp, share, w);
 	if (threadIdx.x == 0) policy_put(g, p, r, a, t, lp, share, w);
-	if (g.dlogits) tile.grad(out, g.V, target, expo(xt, tile.M), coef);
+	if (g.dlogits) tile.grad(out, g.V, target, expo(xt, point(tile.m)), coef);
 }
 template <typename T, int CH, int THREADS>
 __global__ __launch_bounds__(THREADS) void policy_long_kernel(const Rows g, const Policy p) {
@@ -877,13 +897,13 @@ __global__ __launch_bounds__(THREADS) void policy_long_kernel(const Rows g, cons
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
 	const float xt = (float)row[target], share = policy_share<64>(g, p, policy_counts(g, p, flags, counts), a, threadIdx.x & 63);
-	float M, s;
-	block_row_sum<T, CH, THREADS>(row, g.V, red, M, s);
-	const double lp = row_logp(xt, M, s);
+	float m, s;
+	block_row_sum<T, CH, THREADS>(row, g.V, red, m, s);
+	const double lp = row_logp(xt, m, s);
 	PolicyRow w;
 	const float coef = policy_grad(p, a, t, lp, share, w);
 	if (threadIdx.x == 0) policy_put(g, p, r, a, t, lp, share, w);
-	if (g.dlogits) RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, M, -coef / s, coef);
+	if (g.dlogits) RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, m, -coef / s, coef);
 }
 template <typename T, int CH, int LANES, int NC>
 __global__ __launch_bounds__(256) void policy_team_kernel(const Rows g, const Policy p) {
@@ -906,12 +926,12 @@ __global__ __launch_bounds__(256) void policy_team_kernel(const Rows g, const Po
 		}
 		const Walk<LANES> next = now.next(g);
 		if (counts) {
-			float M, s;
-			tile.sum(g.V, lane, M, s);
-			const double lp = row_logp(xt, M, s);
+			float m, s;
+			tile.sum(g.V, lane, m, s);
+			const double lp = row_logp(xt, m, s);
 			PolicyRow w;
 			const float coef = policy_grad(p, now.a, now.t, lp, share, w);
-			if (g.dlogits) tile.grad(out, g.V, lane, target, xt, M, -coef / s, coef);
+			if (g.dlogits) tile.grad(out, g.V, lane, target, xt, m, -coef / s, coef);
 			if (lane == 0) policy_put(g, p, now.r, now.a, now.t, lp, share, w);
 		} else {
 			if (g.dlogits) RowStream<T, CH, LANES>::zero(out, g.V, lane);
@@ -1091,10 +1111,10 @@ extern "C" int novic_token_logprobs_bwd(const void* logits, int type, int64_t ld
 
 // Pair by pair where the pairs alone fill the chip (two workgroups of eight waves a unit), a wave's registers hold a row and the row is long enough for a wave; else row by row, with
 // the pairs between the two launches over the rows.
-constexpr int FUSED_PAIRS = 512;
+constexpr int FUSED_PAIRS = 512, MOST_PAIRS = 1 << 22;  // (a grid's extent in threads is 32 bits)
 bool pair_by_pair(const Rows& g, int type) {
 	const int ch = type == NOVIC_TYPE_F32 ? 4 : 8;
-	return g.A / 2 >= FUSED_PAIRS && 2 * g.T <= PAIR_ROWS && g.V > 64 * ch && g.V <= PAIR_VECTORS * 64 * ch;
+	return g.A / 2 >= FUSED_PAIRS && g.A / 2 <= MOST_PAIRS && 2 * g.T <= PAIR_ROWS && g.V > 64 * ch && g.V <= PAIR_VECTORS * 64 * ch;
 }
 template <typename T, int CH>
 void launch_pairs(const Rows& g, const LogpOut& o, const Pref& q, hipStream_t stream) {

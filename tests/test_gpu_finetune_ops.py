@@ -829,3 +829,73 @@ def test_two_streams_at_once():
 	for a, b in zip(got, eager):
 		for k, (x, y) in enumerate(zip(a, b)):
 			assert torch.equal(x, y) if k != 3 else float((x - y).abs().max()) <= float(y.abs().max()) * 2 ** -10
+
+
+# ---- logits so large that their product with log2 e rounds by whole exponents, or is no number: rows that a mask of -1e10, -1e30 or the type's lowest value leaves empty ------------
+
+def far_rows(n, V, dtype):
+	"""n rows of V logits and a target for each, near a level c: all c; all c but the target, which is c / 2; c with two at c / 2, one of them the target; c with ordinary logits in front."""
+	top = torch.finfo(dtype).max
+	levels = [c for c in (-top, -1e30, -1e10, -1.5e9, -1.3e9, -1e9, -3e4, 3e4, 1e9, 1.3e9, 1.5e9, 1e10, 1e30, top) if abs(c) <= top]
+	r = torch.arange(n, device=DEV)
+	c = torch.tensor(levels, dtype=torch.double, device=DEV)[r % len(levels)].to(dtype)
+	kind = r // len(levels) % 4
+	target = (r * 7919 + 3) % V
+	x = c[:, None].repeat(1, V)
+	half = (c.double() / 2).to(dtype)
+	neg = c < 0
+	for k in (1, 2):
+		pick = (kind == k) & neg  # (with c > 0 the rest would be larger by more than fp32 holds)
+		x[pick, target[pick]] = half[pick]
+		if k == 2:
+			x[pick, (target[pick] + 1) % V] = half[pick]
+	few = min(3, V)
+	pick = (kind == 3) & neg
+	x[pick, :few] = normal(gen(V), n, few, dtype=dtype)[pick]
+	target[pick] = target[pick] % few
+	ref = torch.log_softmax(x.double(), 1)
+	lp = ref.gather(1, target[:, None]).squeeze(1)
+	# The sum is seen from M = fl(m log2 e), up to 2^-24 |M| from the maximum (|M| <= 2.1e9, beyond which m itself is the point): that far is every exponent, its rounding and that of
+	# log2 e are u relative each
+	m = x.double().abs().amax(1).clamp(max=2.1e9)
+	return x, target, ref.exp(), lp, U * (K + 8 + lp.abs() + 4 * 2.0 ** -24 * 1.45 * m)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V", [5, 130, 500, 900, 1500, 5000, 10007, 20001, 70001])
+def test_far_logits(V, dtype):
+	A, T = 8, 14
+	x, target, p, lp, bound = far_rows(A * T, V, dtype)
+	target = target.view(A, T)
+	out, lse = torch.empty(A, T, device=DEV), torch.empty(A * T, device=DEV)
+	ops.token_logprobs(x, target, out, lse=lse)
+	near(out, lp.view(A, T), bound.view(A, T), f"logp, V = {V}")
+	want = torch.logsumexp(x.double(), 1)
+	near(lse, want.float().double(), bound + 2 * U * want.abs(), "lse")
+	onehot = torch.zeros_like(p).scatter_(1, target.view(-1, 1), 1.0)
+	stats, d = torch.empty(4, device=DEV), torch.empty_like(x)
+	ops.policy_loss(x, target, out, torch.full((A,), -float(A * T), device=DEV), stats, dlogits=d)  # ratio 1: the gradient of the sum of the log-probabilities, negated
+	ref = onehot - p
+	near(d, ref, bound[:, None] * (p + onehot) * 3 + half_step(ref, dtype), f"policy gradient, V = {V}")
+	assert abs(float(stats[0]) - A * T) <= 1e-4 * A * T
+	stats, d, n = torch.empty(3, device=DEV), torch.empty_like(x), A // 2
+	margin = torch.empty(n, device=DEV)
+	ops.preference_loss(x, target, out, stats, beta=2.0 * n, kind="square", margin=margin, dlogits=d)  # margin 0: slope -1 / beta^2, n of them, times beta
+	ref = torch.cat([-(onehot - p)[:n * T], (onehot - p)[n * T:]]) / (2.0 * n * n)
+	near(d, ref, bound[:, None] * (p + onehot) / (2.0 * n * n) * 4 + float(margin.abs().max()) * (p + onehot) / n + half_step(ref, dtype), f"preference gradient, V = {V}")
+	assert abs(float(stats[1])) <= 2 * n * 2 * T * U * float(lp.abs().max()) + 1e-30
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [600, 4000])
+def test_far_logits_pair_by_pair(V, dtype):
+	n, T = 560, 3
+	x, target, p, lp, bound = far_rows(2 * n * T, V, dtype)
+	target = target.view(2 * n, T)
+	ref, out, stats, margin, d = lp.float().view(2 * n, T), torch.empty(2 * n, T, device=DEV), torch.empty(3, device=DEV), torch.empty(n, device=DEV), torch.empty_like(x)
+	ops.preference_loss(x, target, ref, stats, beta=1.0, kind="hinge", logp=out, margin=margin, dlogits=d)
+	near(out, lp.view(2 * n, T), bound.view(2 * n, T))
+	onehot = torch.zeros_like(p).scatter_(1, target.view(-1, 1), 1.0)
+	near(margin, torch.zeros(n, device=DEV, dtype=torch.double), (2 * bound + U * lp.abs()).view(2, n, T).sum((0, 2)))
+	want = torch.cat([-(onehot - p)[:n * T], (onehot - p)[n * T:]]) / n  # every margin is below 1
+	near(d, want, bound[:, None] * (p + onehot) / n * 4 + half_step(want, dtype), "gradient")
