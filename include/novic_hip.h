@@ -527,7 +527,7 @@ int novic_layernorm_stats_bwd(const void* dy, int y_type, int64_t lddy, const vo
                               hipStream_t stream);
 
 /* Dropout with a mask that is never stored: y[rows][cols] = (keep ? x * 65536 / (65536 - thr) : 0) (+ resid, of y's type), thr = round(65536 p).  Element i = row * cols + col is
- * kept iff its 16 bits of Philox4x32-10 (key: seed; counter: i / 8 low, high, site, *step -- 0 where step is NULL; half i % 8 of the four words, low half first) are >= thr.
+ * kept iff its 16 bits of Philox4x32-10 (key: seed; counter: i / 8 low, high, site, the low 32 bits of *step -- 0 where step is NULL; half i % 8 of the four words, low half first) are >= thr.
  * The backward pass is the same call on dy without resid.  x and y have one type, or one of them is fp32.  y may be x or resid. */
 int novic_dropout(const void* x, int x_type, int64_t ldx, const void* resid, int64_t ldr, void* y, int y_type, int64_t ldy, int64_t rows, int64_t cols, double p, uint64_t seed,
                   uint32_t site, const int64_t* step, hipStream_t stream);

@@ -7,7 +7,8 @@
 // the backward pass draws it again.  `step` may be a device scalar, so that a replayed graph draws a new mask each time.  The scale uses the probability that 16 bits hold,
 // which keeps the expectation exact.
 //
-// HBM-bound: one generator block (20 32 x 32 -> 64-bit multiplies) serves one 16-byte vector of 16-bit elements.
+// HBM-bound: one generator block (20 32 x 32 -> 64-bit multiplies) serves one 16-byte vector of 16-bit elements.  MI355X: [57344 x 512] bf16 + fp32 residual -> fp32 54 us
+// (294 MB, 5.5 TB/s).
 #include "novic_hip.h"
 #include "rowvec.hpp"
 
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(256) void dropout_rows_kernel(const Args g) {
 			if (e >= 0 && e + 8 <= g.cols) {
 				const RawVec<XT, 8> v = load_vec<XT, 8>(x + e);
 				RawVec<YT, 8> r;
-		float o[8];
+				float o[8];
 				if (RESID) r = load_vec<YT, 8>(resid + e);
 #pragma unroll
 				for (int i = 0; i < 8; ++i) {

@@ -9,7 +9,8 @@
 //
 // HBM-bound: V logits a row in, V gradients a row out.  A row belongs to a workgroup that holds it in registers between the sum and the gradient; padded rows are not read.
 // The exponentials and the sums over the vocabulary are fp32; a log-probability is formed and added up over its sequence in fp64 (a handful of operations a ROW):
-// the losses take differences of sums that nearly cancel.
+// the losses take differences of sums that nearly cancel.  MI355X: gradient of log-probabilities over [4928 x 49408] fp16 134 us (733 MB, 5.5 TB/s); preference step of 4096 pairs of
+// [7 x 6912] bf16 250 us (1249 MB, 5.0 TB/s), policy step of as many rows 218 us (5.7 TB/s).
 #include "novic_hip.h"
 #include "rowvec.hpp"
 
@@ -251,7 +252,13 @@ struct TeamRow {
 	__device__ __forceinline__ static int cut(int c, int V, int lane) { return NC == 1 ? lane * CH : c * STEP - base(c, V); }  // first element of at() .. that counts
 	__device__ __forceinline__ static bool whole(int c, int V) { return (c + 1) * STEP <= V; }
 	__device__ __forceinline__ static bool any(int c, int V) { return c * STEP < V; }
+	// What a row's end needs (NC CH masks of lanes, NC bases) is the same in every row: formed for all rows at once it would fill the scalar registers many times over.  So each use
+	// forms its own, and only the vector at the end has any.
+	__device__ __forceinline__ static void here(int& V, int& lane) {
+		if constexpr (NC > 1) asm volatile("" : "+s"(V), "+v"(lane));
+	}
 	__device__ __forceinline__ void load(const T* row, int V, int lane) {
+		here(V, lane);
 #pragma unroll
 		for (int c = 0; c < NC; ++c) raw[c] = load_vec<T, CH>(elem(row + base(c, V), at(V, lane)));
 	}
@@ -289,6 +296,7 @@ struct TeamRow {
 	__device__ __forceinline__ void sum(int V, int lane, float& m, float& s) {
 		m = top();
 		const Point at_m = at_max(m);
+		here(V, lane);
 		float t = 0.f;
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
@@ -306,6 +314,7 @@ struct TeamRow {
 	__device__ __forceinline__ void grad(T* out, int V, int lane, int target, float xt, float m, float k, float coef) {
 		const Point at_m = at_max(m);
 		asm volatile("" : "+v"(xt));  // (as in RowStream)
+		here(V, lane);
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
 			if (!any(c, V)) continue;
@@ -650,11 +659,13 @@ __global__ __launch_bounds__(1024) void pref_finish_kernel(const Pref g) {
 
 // A pair by one workgroup, loss and gradient.  The pair's rows (at most 64) are lanes' business first: each wave asks for all targets and reference values and knows the rows that
 // count from a ballot.  Those are dealt to the waves in turn; the row that a wave sums last stays in its registers up to its gradient, any others are read again (a pair's
-// time later: out of L2 or the memory-side cache).  Sixteen vectors a lane are what 128 registers hold beside the rest of the kernel.
-constexpr int PAIR_WAVES = 8, PAIR_ROWS = 64, PAIR_VECTORS = 16, PAIR_WEIGHTS = 4096;
-template <typename T, int CH, int NC>
-__global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Rows g, const LogpOut o, const Pref q) {
-	__shared__ double part[3][PAIR_WAVES];
+// time later: out of L2 or the memory-side cache).  Sixteen vectors a lane are what 128 registers hold beside the rest of the kernel.  Bound by the rows in flight: between a pair's
+// reading and its writing stands a barrier, and two workgroups a unit are what covers it.  4096 pairs of 7 + 7 rows of 6912 bf16: 249 us with eight waves, with four 272, with five 261,
+// with six 254.  Second rows kept in LDS instead of read again: 1 % less.
+constexpr int PAIR_ROWS = 64, PAIR_VECTORS = 16, PAIR_WEIGHTS = 4096;
+template <typename T, int CH, int NC, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 4) void pref_pair_kernel(const Rows g, const LogpOut o, const Pref q) {
+	__shared__ double part[3][WAVES];
 	const int i = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, rows = 2 * q.T;
 	const int my_half = lane >= q.T, my_a = my_half ? q.n + i : i, my_t = lane - my_half * q.T;  // lane k stands for row k: the preferred sequence's, then the other's
 	int my_target = -1;
@@ -665,11 +676,11 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 	}
 	double total = 0.0;  // of the weights: few enough are added up by every workgroup (q.total is null), which saves a launch in front of this one
 	if (q.weight && !q.total) {
-		float w[PAIR_WEIGHTS / (PAIR_WAVES * 64)];
+		float w[PAIR_WEIGHTS / (WAVES * 64)];
 #pragma unroll
-		for (int k = 0; k < PAIR_WEIGHTS / (PAIR_WAVES * 64); ++k) w[k] = q.weight[min(k * PAIR_WAVES * 64 + (int)threadIdx.x, q.n - 1)];
+		for (int k = 0; k < PAIR_WEIGHTS / (WAVES * 64); ++k) w[k] = q.weight[min(k * WAVES * 64 + (int)threadIdx.x, q.n - 1)];
 #pragma unroll
-		for (int k = 0; k < PAIR_WEIGHTS / (PAIR_WAVES * 64); ++k) total += k * PAIR_WAVES * 64 + (int)threadIdx.x < q.n ? (double)w[k] : 0.0;
+		for (int k = 0; k < PAIR_WEIGHTS / (WAVES * 64); ++k) total += k * WAVES * 64 + (int)threadIdx.x < q.n ? (double)w[k] : 0.0;
 #pragma unroll
 		for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
 	}
@@ -690,7 +701,7 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 	TeamRow<T, CH, 64, NC> tile;
 	float m = 0.f, s = 1.f, xt = 0.f;
 	int k = 0, r = 0, target = 0;
-	for (int l = wave + (have - 1 - wave) / PAIR_WAVES * PAIR_WAVES; wave < have && l >= 0; l -= PAIR_WAVES) {
+	for (int l = wave + (have - 1 - wave) / WAVES * WAVES; wave < have && l >= 0; l -= WAVES) {
 		k = nth(counted, l), r = row_of(k), target = of_lane(my_target, k);
 		const T* row = (const T*)g.logits + (long long)r * g.ldl;
 		tile.load(row, g.V, lane);
@@ -703,29 +714,31 @@ __global__ __launch_bounds__(PAIR_WAVES * 64, 4) void pref_pair_kernel(const Row
 		part[1][wave] = u[1];
 		part[2][wave] = total;
 	}
-	for (int l = PAIR_WAVES - 1 - wave; l < none; l += PAIR_WAVES) {
+	for (int l = WAVES - 1 - wave; l < none; l += WAVES) {
 		const int kz = nth(others, l), rz = row_of(kz);
 		if (g.dlogits) RowStream<T, CH, 64>::zero((T*)g.dlogits + (long long)rz * g.ldd, g.V, lane);
 		if (lane == 0) put_logp(o, rz, kz >= q.T ? q.n + i : i, kz >= q.T ? kz - q.T : kz, false, 0.0, 0.f, 1.f);
 	}
 	__syncthreads();
-	u[0] = u[1] = total = 0.0;
+	u[0] = part[0][lane & (WAVES - 1)];  // (a wave's sum a lane: all in every lane's registers would be the most that the kernel holds beside its row)
+	u[1] = part[1][lane & (WAVES - 1)];
+	total = part[2][lane & (WAVES - 1)];
 #pragma unroll
-	for (int w = 0; w < PAIR_WAVES; ++w) {
-		u[0] += part[0][w];
-		u[1] += part[1][w];
-		total += part[2][w];
+	for (int o = WAVES / 2; o > 0; o >>= 1) {
+		u[0] += __shfl_xor(u[0], o, 64);
+		u[1] += __shfl_xor(u[1], o, 64);
+		total += __shfl_xor(total, o, 64);
 	}
 	if (!q.weight) total = (double)q.n;
 	else if (q.total) total = *q.total;
 	const double z = pref_margin(q, u[0], u[1]);
-	if (threadIdx.x == PAIR_WAVES * 64 - 1) pref_terms(q, i, z);  // (the last wave: it has the fewest rows)
+	if (threadIdx.x == WAVES * 64 - 1) pref_terms(q, i, z);  // (the last wave: it has the fewest rows)
 	if (!g.dlogits) return;
 	const float c = pref_slope(q, i, z) * pref_scale(q, total);
 	if (wave >= have) return;
 	float coef = k >= q.T ? -c : c;
 	tile.grad((T*)g.dlogits + (long long)r * g.ldd, g.V, lane, target, xt, m, -coef / s, coef);
-	for (int l = wave + PAIR_WAVES; l < have; l += PAIR_WAVES) {
+	for (int l = wave + WAVES; l < have; l += WAVES) {
 		k = nth(counted, l), r = row_of(k), target = of_lane(my_target, k);
 		const T* row = (const T*)g.logits + (long long)r * g.ldl;
 		const float2 norm = o.norm[r];  // (written by this wave)
@@ -1116,13 +1129,22 @@ bool pair_by_pair(const Rows& g, int type) {
 	const int ch = type == NOVIC_TYPE_F32 ? 4 : 8;
 	return g.A / 2 >= FUSED_PAIRS && g.A / 2 <= MOST_PAIRS && 2 * g.T <= PAIR_ROWS && g.V > 64 * ch && g.V <= PAIR_VECTORS * 64 * ch;
 }
+// Eight waves, of which two workgroups are resident; sixteen, which read fewer rows twice, for more than sixteen long rows a pair (bf16, 6912 columns, pairs of 2 T rows: T = 32 459 us
+// with eight, 396 with sixteen; T = 16 402 and 368; T = 7 302 and 321; T = 3 253 and 363; 2000 columns, T = 16: 228 and 230).
 template <typename T, int CH>
 void launch_pairs(const Rows& g, const LogpOut& o, const Pref& q, hipStream_t stream) {
-	const dim3 grid((unsigned)q.n), block(PAIR_WAVES * 64);
-	if (g.V <= 4 * 64 * CH) pref_pair_kernel<T, CH, 4><<<grid, block, 0, stream>>>(g, o, q);
-	else if (g.V <= 8 * 64 * CH) pref_pair_kernel<T, CH, 8><<<grid, block, 0, stream>>>(g, o, q);
-	else if (g.V <= 12 * 64 * CH) pref_pair_kernel<T, CH, 12><<<grid, block, 0, stream>>>(g, o, q);
-	else pref_pair_kernel<T, CH, PAIR_VECTORS><<<grid, block, 0, stream>>>(g, o, q);
+	const dim3 grid((unsigned)q.n), eight(8 * 64), sixteen(16 * 64);
+	if (g.V <= 4 * 64 * CH) {
+		pref_pair_kernel<T, CH, 4, 8><<<grid, eight, 0, stream>>>(g, o, q);
+	} else if (g.V <= 8 * 64 * CH) {
+		pref_pair_kernel<T, CH, 8, 8><<<grid, eight, 0, stream>>>(g, o, q);
+	} else if (g.V <= 12 * 64 * CH) {
+		if (2 * g.T <= 16) pref_pair_kernel<T, CH, 12, 8><<<grid, eight, 0, stream>>>(g, o, q);
+		else pref_pair_kernel<T, CH, 12, 16><<<grid, sixteen, 0, stream>>>(g, o, q);
+	} else {
+		if (2 * g.T <= 16) pref_pair_kernel<T, CH, PAIR_VECTORS, 8><<<grid, eight, 0, stream>>>(g, o, q);
+		else pref_pair_kernel<T, CH, PAIR_VECTORS, 16><<<grid, sixteen, 0, stream>>>(g, o, q);
+	}
 }
 
 // workspace: diff [2n T] fp64, each [2][n] fp64, norm [2n T] float2, coef [2n], total fp64, scale

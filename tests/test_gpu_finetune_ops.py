@@ -899,3 +899,10 @@ def test_far_logits_pair_by_pair(V, dtype):
 	near(margin, torch.zeros(n, device=DEV, dtype=torch.double), (2 * bound + U * lp.abs()).view(2, n, T).sum((0, 2)))
 	want = torch.cat([-(onehot - p)[:n * T], (onehot - p)[n * T:]]) / n  # every margin is below 1
 	near(d, want, bound[:, None] * (p + onehot) / n * 4 + half_step(want, dtype), "gradient")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,T,V", [(513, 9, 5000), (512, 20, 3000), (515, 32, 4001), (512, 8, 4096), (512, 9, 8192)])
+def test_preference_many_long_rows(n, T, V, dtype):
+	"""Pairs of more long rows than their workgroup has waves."""
+	test_preference(n, T, V, 3, 1, dtype, "sigmoid", 0.1, 0.3)
