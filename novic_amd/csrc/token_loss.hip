@@ -1162,7 +1162,7 @@ extern "C" int novic_preference_loss(const void* logits, int type, int64_t ldl, 
 	NOVIC_CHECK(!bad, bad);
 	NOVIC_CHECK(ref && stats && ldref >= T && (!logp || ldo >= T), "novic_preference_loss: ref [2n][ldref >= T], stats [3]");
 	NOVIC_CHECK(kind == NOVIC_PREF_SIGMOID || kind == NOVIC_PREF_HINGE || kind == NOVIC_PREF_SQUARE, "novic_preference_loss: unknown kind");
-	NOVIC_CHECK(beta > 0.0 && smoothing >= 0.0 && smoothing < 0.5 && (smoothing == 0.0 || kind == NOVIC_PREF_SIGMOID), "novic_preference_loss: beta > 0; smoothing in [0, 0.5), with the sigmoid form only");
+	NOVIC_CHECK(beta > 0.0 && beta < INFINITY && smoothing >= 0.0 && smoothing < 0.5 && (smoothing == 0.0 || kind == NOVIC_PREF_SIGMOID), "novic_preference_loss: a finite beta > 0; smoothing in [0, 0.5), with the sigmoid form only");
 	NOVIC_CHECK(ws && ws_bytes >= novic_preference_loss_ws(n, T), "novic_preference_loss: the workspace is smaller than novic_preference_loss_ws says");
 	NOVIC_APART("novic_preference_loss",
 	            NOVIC_SPANS(dlogits_span(g, type), vector_span(stats, 12), vector_span(margin, 4LL * n), token_span(g, logp, ldo), vector_span(ws, novic_preference_loss_ws(n, T))),

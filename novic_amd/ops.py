@@ -1012,8 +1012,8 @@ def layernorm_stats_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: Optional[tor
 	rows, E = x.shape
 	dev, xt = x.device, x.dtype
 	po, ldo = _matrix(out, "out", dev, rows, E, _TYPE if xt is torch.float32 else (xt,))
-	if not 1 <= E <= 16384:
-		raise ValueError(f"layernorm_stats_fwd: 1 <= width <= 16384, got {E}")
+	if not 1 <= E <= 16384 or rows >= 1 << 31:
+		raise ValueError(f"layernorm_stats_fwd: 1 <= width <= 16384 and fewer than 2^31 rows, got {rows} x {E}")
 	_enqueue("novic_layernorm_stats_fwd", dev, px, _TYPE[xt], ldx, _vector(_given(gamma, "gamma"), "gamma", dev, E), _vector(beta, "beta", dev, E), po, _TYPE[out.dtype], ldo,
 	         _vector(mean, "mean", dev, rows), _vector(rstd, "rstd", dev, rows), rows, E, eps)
 	return out
@@ -1029,8 +1029,8 @@ def layernorm_stats_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, 
 	pdy, lddy = _matrix(dy, "dy", dev, rows, E, _TYPE if xt is torch.float32 else (xt,))
 	pdx, lddx = _matrix(dx, "dx", dev, rows, E, (xt,))
 	pin, ldi = _matrix(dx_in, "dx_in", dev, rows, E, (xt,)) if dx_in is not None else (0, 0)
-	if not 1 <= E <= 16384:
-		raise ValueError(f"layernorm_stats_bwd: 1 <= width <= 16384, got {E}")
+	if not 1 <= E <= 16384 or rows >= 1 << 31:
+		raise ValueError(f"layernorm_stats_bwd: 1 <= width <= 16384 and fewer than 2^31 rows, got {rows} x {E}")
 	pdg, pdb = _vector(dgamma, "dgamma", dev, E), _vector(dbeta, "dbeta", dev, E)
 	xi, yi = _TYPE[xt], _TYPE[dy.dtype]
 	need = _ws_bytes("novic_layernorm_stats_bwd_ws", rows, E, xi, yi) if pdg or pdb else 0
@@ -1080,8 +1080,8 @@ def _token_rows(logits, target, pad):
 	R, V = logits.shape
 	if R != A * T:
 		raise ValueError(f"logits: one row for each of the {A} x {T} target positions, got {R}")
-	if V < 1 or R >= 1 << 31:
-		raise ValueError("token rows: a vocabulary of at least one, at most 2^31 - 1 rows")
+	if not 1 <= V <= 1 << 28 or R >= 1 << 31:
+		raise ValueError("token rows: a vocabulary of 1 to 2^28, at most 2^31 - 1 rows")
 	pp, ldp = _matrix(pad, "pad", dev, A, T, _MASKS) if pad is not None else (0, 0)
 	return dev, A, T, V, (pl, _TYPE[logits.dtype], ldl, pt, target.element_size(), ldt, pp, ldp)
 
@@ -1139,8 +1139,8 @@ def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref: torch.Tenso
 	n = A // 2
 	if kind not in PREFERENCE_KINDS:
 		raise ValueError(f"preference_loss: kind is one of {', '.join(PREFERENCE_KINDS)}, got {kind!r}")
-	if not beta > 0.0 or not 0.0 <= smoothing < 0.5 or (smoothing != 0.0 and kind != "sigmoid"):
-		raise ValueError("preference_loss: beta > 0, smoothing in [0, 0.5) and with the sigmoid form only")
+	if not 0.0 < beta < float("inf") or not 0.0 <= smoothing < 0.5 or (smoothing != 0.0 and kind != "sigmoid"):
+		raise ValueError("preference_loss: a finite beta > 0, smoothing in [0, 0.5) and with the sigmoid form only")
 	pref, ldref = _matrix(ref, "ref", dev, A, T, _F32)
 	plp, ldo = _optional(logp, "logp", dev, A, T, _F32)
 	pd, ldd = _optional(dlogits, "dlogits", dev, A * T, V, (logits.dtype,))

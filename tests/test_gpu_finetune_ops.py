@@ -906,3 +906,18 @@ def test_far_logits_pair_by_pair(V, dtype):
 def test_preference_many_long_rows(n, T, V, dtype):
 	"""Pairs of more long rows than their workgroup has waves."""
 	test_preference(n, T, V, 3, 1, dtype, "sigmoid", 0.1, 0.3)
+
+
+def test_counts_beyond_their_types_are_refused():
+	"""Row and column counts that a C int does not hold are refused, not cut to their low 32 bits."""
+	x = torch.empty((1 << 32) + 5, 1, dtype=BF16, device=DEV)
+	one = torch.ones(1, device=DEV)
+	with pytest.raises(ValueError):
+		ops.layernorm_stats_fwd(x, one, None, x)
+	with pytest.raises(ValueError):
+		ops.layernorm_stats_bwd(x, x, one, torch.empty(5, device=DEV), torch.empty(5, device=DEV), x)
+	row, t = x.view(1, -1), torch.zeros(1, 1, dtype=torch.int64, device=DEV)
+	with pytest.raises(ValueError):
+		ops.token_logprobs(row, t, torch.empty(1, 1, device=DEV))
+	with pytest.raises(ValueError):
+		ops.preference_loss(torch.zeros(2, 4, device=DEV), t.repeat(2, 1), torch.zeros(2, 1, device=DEV), torch.empty(3, device=DEV), beta=float("inf"))
