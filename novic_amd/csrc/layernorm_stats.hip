@@ -7,7 +7,7 @@
 // read), statistics and sums in fp32.  A row belongs to a team of 16, 64 or 256 lanes, the smallest that holds it in about four vectors a lane, or of 512, whose lanes take up to
 // eight (with 1024 lanes a lane has 128 registers: 5 % faster backward at 16384 columns, but one type's form spills, and 6 to 40 % slower forward).  What is read once is loaded, and
 // gradients are stored, past the caches.  MI355X: forward [57344 x 512] fp32 -> bf16 30.4 us (5.8 TB/s), [65792 x 1280] bf16 66 us (5.1); backward [65792 x 1280] bf16 with both
-// affine gradients and the residual's added 121 us (5.6 TB/s, of it 7 us in the reduction of the partial rows; without those hints 132).
+// affine gradients and the residual's added 121 us (5.6 TB/s, of it 5 us in the reduction of the partial rows; without those hints 132).
 #include "novic_hip.h"
 #include "rowvec.hpp"
 

@@ -994,11 +994,13 @@ __global__ __launch_bounds__(256) void policy_slices_kernel(const Policy p) {
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------------------------------------
 // Rows in registers, by workgroup; longer ones take the form that reads a row twice (its second pass comes out of L2 / the memory-side cache).
+// (512 lanes with eight vectors each, against 1024 with four: policy step of 315 MB of bf16 logits, 17000 columns 158 and 231 us, 24000 124 and 181, 32700 127 and 164.  1024 with eight
+// against reading twice: 40000 columns 170 and 171, 50000 164 and 176, 65000 154 and 176.)
 #define NOVIC_ROW_SHAPES(V, REG, LONG)                                                                     \
 	if (V <= 512 * CH) { constexpr int TH = 256, NC = 2; REG; }                                              \
 	else if (V <= 1024 * CH) { constexpr int TH = 256, NC = 4; REG; }                                        \
 	else if (V <= 2048 * CH) { constexpr int TH = 256, NC = 8; REG; }                                        \
-	else if (V <= 4096 * CH) { constexpr int TH = 1024, NC = 4; REG; }                                       \
+	else if (V <= 4096 * CH) { constexpr int TH = 512, NC = 8; REG; }                                        \
 	else if (V <= 8192 * CH) { constexpr int TH = 1024, NC = 8; REG; }                                       \
 	else { constexpr int TH = 1024; LONG; }
 constexpr int SHORT = 128;
@@ -1011,9 +1013,9 @@ constexpr int SHORT = 128;
 	else if (V <= 8 * 64 * CH) { constexpr int L = 64, NC = MOST < 8 ? MOST : 8; CALL; }                     \
 	else { constexpr int L = 64, NC = MOST; CALL; }
 
-// Short rows go by team: a workgroup for each is mostly its own start and end ([104857 x 1500] bf16, log-probabilities 82 us by wave, 274 by workgroup; policy with gradient 158 and
-// 223; gradient 154 and 211).  Beyond four vectors a lane a workgroup's many registers win where there are gradients to store (4000 columns: 121 and 114 us); without, a wave
-// keeps up to sixteen, given rows enough for all waves (6000 columns: 64 and 84 us; at 1500 rows 9.1 and 8.1).
+// Short rows go by team: a workgroup for each is mostly its own start and end ([104857 x 1500] bf16, log-probabilities 84 us by wave, 274 by workgroup; policy with gradient 151 and
+// 223; gradient 149 and 211).  Beyond four vectors a lane a workgroup's many registers win where there are gradients to store (4000 columns: 121 and 114 us); without, a wave
+// keeps up to sixteen, given rows enough for all waves (6000 columns: 55 and 84 us; at 1500 rows 8.4 and 8.1).
 template <int CH>
 bool by_team(const Rows& g, bool stores) { return g.V <= 4 * 64 * CH || (!stores && g.V <= 16 * 64 * CH && (long long)g.A * g.T >= 4096); }
 template <int LANES>
