@@ -769,9 +769,9 @@ __global__ __launch_bounds__(256) void policy_count_kernel(const Rows g, const P
 	__shared__ int red[8];
 	const int lane = threadIdx.x % lanes, teams = 256 / lanes;
 	int rows = 0, seqs = 0;
-	for (int a = blockIdx.x * teams + threadIdx.x / lanes; a < g.A; a += gridDim.x * teams) {
+	for (unsigned a = blockIdx.x * teams + threadIdx.x / lanes; a < (unsigned)g.A; a += gridDim.x * teams) {  // (unsigned: what is behind the last may be beyond 2^31)
 		int n = 0;
-		for (int t = lane; t < g.T; t += lanes) n += counted_target(g, a, t) >= 0;
+		for (unsigned t = lane; t < (unsigned)g.T; t += lanes) n += counted_target(g, a, t) >= 0;
 		for (int o = lanes / 2; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
 		if (lane == 0) {
 			p.len[a] = n;

@@ -48,3 +48,16 @@ def test_layernorm_backward_of_the_most_rows():
 	for s in pieces(MOST):
 		assert bool((dx[s] == -x[s] * x[s] * dy[s]).all()), s
 	assert float(dgamma) == float((last * x[-40_000:, 0].long()).sum()) and float(dbeta) == float(last.sum())
+
+
+def test_policy_of_the_most_sequences():
+	"""2^31 - 1 sequences of one position, one logit: a sequence's count is taken in steps that end beyond 2^31.  The log-probability is 0; ratio 1, advantages only at the end."""
+	logits, target = torch.zeros(MOST, 1, dtype=BF16, device=DEV), torch.zeros(MOST, 1, dtype=torch.int32, device=DEV)
+	target[1::2] = -1  # every other position does not count
+	old, adv, stats = torch.zeros(MOST, 1, device=DEV), torch.zeros(MOST, device=DEV), torch.empty(4, device=DEV)
+	adv[-1000:] = -3.0
+	count = (MOST + 1) // 2
+	for per_seq in (False, True):
+		ops.policy_loss(logits, target, old, adv, stats.fill_(7), per_sequence=per_seq)
+		want = 3.0 * 500 / count
+		assert abs(float(stats[0]) - want) <= 8 * U * want and float(stats[1]) == 0 and float(stats[2]) == 0 and float(stats[3]) == float(torch.tensor(float(count)))
