@@ -1180,12 +1180,13 @@ class PrefixedIterDecoder(EmbeddingDecoder):
 	# embedding, clipped policy steps on sampled labels.  Gradients are ACCUMULATED into the flat gradient buffer, as by forward_backward; the optimizer step is the caller's. ----
 	def token_logprobs(self, embed, target, target_padding) -> torch.Tensor:
 		"""fp32 log-probabilities of the target tokens, target's shape, 0 where target_padding says so: what a frozen decoder contributes as ref_logprobs and a sampling one as
-		old_logprobs.  target: [B][C], or [2][B][C] for the two labels of each preference (no dropout, whatever the mode)."""
+		old_logprobs.  target: [B][C], or [2][B][C] for the two labels of each preference (no dropout, whatever the mode).  Its activations have a workspace of their own: a loss of
+		forward() whose backward() is still to come keeps its own."""
 		flat, pad, rep = self._finetune_inputs(target, target_padding)
 		out = torch.empty(flat.shape, dtype=torch.float32, device=flat.device)
 		if not out.numel():
 			return out.view(target.shape)
-		sv = self._run_forward(embed, flat, pad, None, rep, rep > 1, only_pred=False, train=False, drop=Dropout(0.0, 0, 0), tag="fwd")
+		sv = self._run_forward(embed, flat, pad, None, rep, rep > 1, only_pred=False, train=False, drop=Dropout(0.0, 0, 0), tag="logprobs")
 		ops.token_logprobs(self._buf(sv, "logits")[:, :self.target_config.vocab_size], flat, out, pad=pad)
 		return out.view(target.shape)
 
