@@ -613,6 +613,8 @@ class PrefixedIterDecoder(EmbeddingDecoder):
 		M = A * S
 		if S > 32:
 			raise ValueError(f"Sequence length {S} exceeds the 32 positions the fused attention kernel holds in registers")
+		if self._saved is not None and self._saved.tag == tag:
+			self._saved = None  # its activations are about to be written over: a backward() that still waits for them raises
 		self.flat_shadow()
 		ws = self._ws
 		g = lambda name, shape, dtype, zero=False: ws.get(f"{tag}:{name}", shape, dtype, dev, zero)

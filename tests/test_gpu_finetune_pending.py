@@ -38,3 +38,17 @@ def test_log_probabilities_between_a_loss_and_its_gradient(pending, rows):
 	for (k, _), a, b in zip(model.named_parameters(), torch.autograd.grad(loss, list(model.parameters())), grads):
 		# float atomics of the weight gradients: at most 64 rows' terms in another order, 64 * 2^-24 of their absolute sum, allowed to be 64 times the largest gradient
 		assert float((a - b).abs().max()) <= 2.0 ** -12 * float(b.abs().max()), k
+
+
+@pytest.mark.parametrize("rows", [8, 3])
+def test_a_forward_without_gradients_ends_the_waiting_one(pending, rows):
+	"""forward() has one workspace: another pass through it, without gradients too, writes over the activations, and the gradient that still waits for them is refused."""
+	model, forward, grads, (embed, target, pad, _) = pending
+	loss = forward()
+	with torch.no_grad():
+		model(embed[:rows], target[:rows], pad[:rows], None, True, False, False, None)
+	with pytest.raises(RuntimeError, match="before the next forward"):
+		loss.backward()
+	again = torch.autograd.grad(forward(), list(model.parameters()))  # and the next pair is whole
+	for (k, _), a, b in zip(model.named_parameters(), again, grads):
+		assert float((a - b).abs().max()) <= 2.0 ** -12 * float(b.abs().max()), k
