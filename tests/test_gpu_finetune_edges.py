@@ -61,3 +61,59 @@ def test_policy_of_the_most_sequences():
 		ops.policy_loss(logits, target, old, adv, stats.fill_(7), per_sequence=per_seq)
 		want = 3.0 * 500 / count
 		assert abs(float(stats[0]) - want) <= 8 * U * want and float(stats[1]) == 0 and float(stats[2]) == 0 and float(stats[3]) == float(torch.tensor(float(count)))
+
+
+@pytest.mark.parametrize("per_seq", [False, True])
+@pytest.mark.parametrize("V,dtype", [(5, F32), (100, BF16), (1500, F16), (1500, F32), (5000, BF16), (40_000, F32), (70_001, BF16)])
+def test_policy_of_large_differences(V, dtype, per_seq):
+	"""Ratios and KL terms beyond fp32 (88.7) and beyond fp64 (709) are finite gradients where what they are multiplied with is zero or small: advantages of 0, a KL coefficient
+	of 0 (the KL is watched, not trained on), small coefficients; against the definition in 64 bits, where a zero factor leaves the term out."""
+	g = torch.Generator(device=DEV).manual_seed(V)
+	x = (2.0 * torch.randn(8, V, generator=g, device=DEV)).to(dtype)
+	target = torch.randint(0, V, (4, 2), generator=g, device=DEV)
+	lse = torch.logsumexp(x.double(), 1)
+	lp = (x.double().gather(1, target.view(-1, 1)).squeeze(1) - lse).view(4, 2)
+	p = (x.double() - lse[:, None]).exp()
+	onehot = torch.zeros_like(p).scatter_(1, target.view(-1, 1), 1.0)
+	d_old = torch.tensor([[100.0, 1000.0], [60.0, -100.0], [95.0, 0.1], [-0.5, 0.5]], device=DEV, dtype=torch.double)
+	d_ref = torch.tensor([[100.0, -100.0], [1000.0, 0.3], [95.0, -1000.0], [2.0, 0.0]], device=DEV, dtype=torch.double)
+	old, ref = (lp - d_old).float(), (lp + d_ref).float()
+	adv = torch.tensor([[0.0, 0.0], [-1e-10, 2.0], [-1e-20, 1.0], [-1.0, -0.0]], device=DEV)
+	share = torch.full((4, 2), 1 / 8, device=DEV, dtype=torch.double)  # (all positions count: both means are the same)
+	for kl in (0.0, 1e-30):
+		rr = torch.where(ref - lp > 700, lp + 90.0, ref.double()).float() if kl else ref
+		stats, d, out = torch.empty(4, device=DEV), torch.empty_like(x), torch.empty(4, 2, device=DEV)
+		ops.policy_loss(x, target, old, adv, stats, clip=(0.2, 0.3), ref=rr, kl_coef=kl, per_sequence=per_seq, dlogits=d, logp=out)
+		q, dd, a = (lp - old.double()).exp(), rr.double() - lp, adv.double()
+		cut = ((a > 0) & (q > 1.3)) | ((a < 0) & (q < 0.8))
+		zero = torch.zeros((), device=DEV, dtype=torch.double)
+		gain = torch.where(a == 0, zero, torch.where(cut, torch.where(a > 0, 1.3, 0.8), q) * a)
+		term = torch.expm1(dd) - dd
+		coef = torch.where(cut, zero, -torch.where(a == 0, zero, q * a)) - (kl * torch.expm1(dd) if kl else zero)
+		each = -gain + (kl * term if kl else zero)
+		want = (coef * share).view(-1, 1) * (onehot - p)
+		# a log-probability is off by (96 + 20) U at most (96 additions, its exponents' distances), its ratio and exp(d) by that much relative, so that the slope expm1(d) of the KL
+		# term is off by exp(d) times that; 32 U for all other roundings
+		off = 150 * U
+		bound = ((coef.abs() + (kl * dd.exp() if kl else zero)) * share).view(-1, 1) * off * (onehot + p) * 2 + want.abs() * (torch.finfo(dtype).eps / 2 + 8 * U) + torch.finfo(dtype).smallest_normal
+		held = want.abs() <= torch.finfo(dtype).max  # (infinite where fp16 does not hold it)
+		assert torch.isfinite(d[held]).all() and not d.isnan().any()
+		assert bool(((d.double() - want).abs() <= bound)[held].all()), (kl, float(((d.double() - want).abs() - bound)[held].max()))
+		loss = float((each * share).sum())
+		assert math.isfinite(float(stats[0])) and abs(float(stats[0]) - loss) <= off * float((each.abs() * share).sum())
+		assert float(stats[2]) == float((cut * share).sum()) and float(stats[3]) == 8
+		mean = float((term * share).sum())  # (infinite where fp32 does not hold it)
+		assert math.isinf(float(stats[1])) if mean > 3.4028236e38 else abs(float(stats[1]) - mean) <= off * float(((term.abs() + dd.abs()) * share).sum())
+
+
+def test_policy_of_an_excluded_target():
+	"""A target whose logit is -inf: log-probability -inf, ratio 0.  With a KL coefficient of 0 (or no reference) the row's gradient is that of the ratio, a zero, and the loss is finite."""
+	x = torch.zeros(2, 300, device=DEV)
+	x[0, 7] = float("-inf")
+	target, old, adv = torch.tensor([[7, 7]], device=DEV), torch.full((1, 2), -6.0, device=DEV), torch.full((1,), -1.5, device=DEV)
+	for ref in (None, torch.full((1, 2), -6.0, device=DEV)):
+		stats, d = torch.empty(4, device=DEV), torch.full_like(x, 7.0)
+		ops.policy_loss(x, target, old, adv, stats, ref=ref, dlogits=d)
+		assert not d[0].any() and torch.isfinite(d).all() and bool(d[1, 7] != 0)
+		q = math.exp(6.0) / 300  # the second row's ratio, 1.34: above the range, but the advantage is negative; the first row's is 0 and held at 0.8
+		assert abs(float(stats[0]) - (q + 0.8) * 1.5 / 2) <= 1e-5 and float(stats[2]) == 0.5
