@@ -534,7 +534,8 @@ int novic_dropout(const void* x, int x_type, int64_t ldx, const void* resid, int
 
 /* Token rows of the losses: logits [A T][ldl >= V], 1 <= V <= 2^28, target [A][ldt] token ids, pad [A][ldp] (may be NULL; 1 = padded).  Row a T + t counts if it is not padded and its target lies
  * in [0, V); other rows' logits are not read, their outputs are zeros.  Columns V .. of dlogits are left as they are.  dlogits may be logits.
- * logp [A][ldo] = x_target - logsumexp(x); lse [A T] (may be NULL).  Backward: dlogits = grad(a, t) ([v = target] - exp(x - lse)), grad(a, t) = grad[a grad_lda + t grad_ldt]. */
+ * logp [A][ldo] = x_target - logsumexp(x); lse [A T] (may be NULL).  Backward: dlogits = grad(a, t) ([v = target] - exp(x - lse)), grad(a, t) = grad[a grad_lda + t grad_ldt].
+ * Where |lse| > 256 and lse is the rounding of the row's own log-sum-exp, that one stands for it, unrounded (at 1e9 the rounding is more than log V). */
 int novic_token_logprobs(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int A, int T, int V,
                          float* logp, int64_t ldo, float* lse, hipStream_t stream);
 int novic_token_logprobs_bwd(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int A, int T, int V,

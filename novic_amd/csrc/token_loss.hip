@@ -386,12 +386,13 @@ __device__ __forceinline__ void put_logp(const LogpOut& o, int r, int a, int t, 
 	if (o.norm) o.norm[r] = counts ? make_float2(m, 1.f / s) : make_float2(0.f, 0.f);
 }
 
-template <typename T, int CH, int THREADS>
+template <typename T, int CH, int THREADS, int UNROLL = 4>
 __device__ __forceinline__ void block_row_sum(const T* row, int V, float* red, float& m, float& s) {
+	typedef RowStream<T, CH, THREADS, UNROLL> Stream;
 	float tm, ts;
-	RowStream<T, CH, THREADS>::sum(row, V, threadIdx.x, tm, ts);
+	Stream::sum(row, V, threadIdx.x, tm, ts);
 	m = block_max<THREADS>(tm, red);
-	s = block_sum<THREADS>(RowStream<T, CH, THREADS>::scaled(tm, ts, m), red + THREADS / 64);
+	s = block_sum<THREADS>(Stream::scaled(tm, ts, m), red + THREADS / 64);
 }
 __device__ __forceinline__ double row_logp(float xt, float m, float s) { return ((double)xt - from_point(m)) - log_wide(s); }
 template <typename T, int CH, int THREADS>
@@ -442,8 +443,15 @@ struct GradIn {
 	long long lda, ldt;
 	const float* scale;   // device scalar or null
 };
-// dlogits = k exp(x - m) + (coef at the target)
-__device__ __forceinline__ void grad_terms(const GradIn& in, int r, int a, int t, float& m, float& k, float& coef) {
+// An lse beyond COARSE has lost what its rounding (2^-16 and more) takes from every probability, at 1e9 all of log V: there the row's sum is formed again, at a second read, and used if
+// lse is its rounding (one that is not, such as that of a vocabulary of which these are some columns, stands as it is).  By one vector at a time: such rows are rare, and more would
+// take registers from the others.
+constexpr float COARSE = 256.f;
+// (lse and the point from which s is seen are each off by 2^-24 of themselves, their difference rounds once more)
+__device__ __forceinline__ bool rounds_to(float m, float s, float lse) { return fabsf((m - lse) + logf(s)) <= fabsf(lse) * 0x1p-22f; }
+// dlogits = k exp(x - m) + (coef at the target); sums(m, s): the row's maximum and sum
+template <typename Sums>
+__device__ __forceinline__ void grad_terms(const GradIn& in, int r, int a, int t, float& m, float& k, float& coef, Sums sums) {
 	coef = in.grad[a * in.lda + t * in.ldt];
 	if (in.scale) coef *= *in.scale;
 	k = -coef;
@@ -451,14 +459,24 @@ __device__ __forceinline__ void grad_terms(const GradIn& in, int r, int a, int t
 		const float2 n = in.norm[r];
 		m = n.x;
 		k *= n.y;
-	} else {
-		m = in.lse[r];
-		const Point at_m = point(m);
-		k *= __builtin_amdgcn_exp2f(-fmaf(m, at_m.L, -at_m.M));  // (what the point's rounding took: s is what lse says, seen from M)
+		return;
 	}
+	const float lse = in.lse[r];
+	if (fabsf(lse) > COARSE) {
+		float s;
+		sums(m, s);
+		if (rounds_to(m, s, lse)) {
+			k /= s;
+			return;
+		}
+	}
+	m = lse;
+	const Point at_m = point(m);
+	k *= __builtin_amdgcn_exp2f(-fmaf(m, at_m.L, -at_m.M));  // (what the point's rounding took: s is what lse says, seen from M)
 }
 template <typename T, int CH, int THREADS>
 __global__ __launch_bounds__(THREADS) void logp_grad_kernel(const Rows g, const GradIn in) {
+	__shared__ float red[2 * THREADS / 64];
 	const int r = row_index(g);
 	if (r < 0) return;
 	const int a = r / g.T, t = r - a * g.T;
@@ -470,7 +488,7 @@ __global__ __launch_bounds__(THREADS) void logp_grad_kernel(const Rows g, const 
 	}
 	const T* row = (const T*)g.logits + (long long)r * g.ldl;
 	float m, k, coef;
-	grad_terms(in, r, a, t, m, k, coef);
+	grad_terms(in, r, a, t, m, k, coef, [&](float& top, float& s) { block_row_sum<T, CH, THREADS, 1>(row, g.V, red, top, s); });
 	const float xt = (float)row[target];  // (used by the lane that owns the target alone, which loads it before it writes there: out may be row)
 	RowStream<T, CH, THREADS>::grad(row, out, g.V, threadIdx.x, target, xt, m, k, coef);
 }
@@ -487,9 +505,15 @@ __global__ __launch_bounds__(256) void logp_grad_team_kernel(const Rows g, const
 		if (target < 0) {
 			Stream::zero(out, g.V, lane);
 		} else {
-			float m, k, coef;
-			grad_terms(in, now.r, now.a, now.t, m, k, coef);
 			const T* row = (const T*)g.logits + (long long)now.r * g.ldl;
+			float m, k, coef;
+			grad_terms(in, now.r, now.a, now.t, m, k, coef, [&](float& top, float& s) {
+				typedef RowStream<T, CH, LANES, 1> Slow;
+				float tm, ts;
+				Slow::sum(row, g.V, lane, tm, ts);
+				top = team_max<LANES>(tm);
+				s = team_sum<LANES>(Slow::scaled(tm, ts, top));
+			});
 			Stream::grad(row, out, g.V, lane, target, (float)row[target], m, k, coef);
 		}
 		now = next;

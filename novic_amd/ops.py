@@ -1118,7 +1118,8 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, out: torch.Tensor
 
 def token_logprobs_bwd(logits: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor, dlogits: torch.Tensor, *, pad: Optional[torch.Tensor] = None):
 	"""dlogits (logits' type, may be logits) = grad[a][t] ([v = target] - exp(logits - lse)); zeros where a position does not count (novic_token_logprobs_bwd).  grad: fp32 [A][T], or
-	[A] for a gradient that all positions of a sequence share (the backward of a sequence's sum)."""
+	[A] for a gradient that all positions of a sequence share (the backward of a sequence's sum).  lse: as token_logprobs wrote it; beyond 256, where its rounding would show in every
+	probability, the row's sum is formed again (a second read of such rows)."""
 	dev, A, T, V, head = _token_rows(logits, target, pad)
 	pd, ldd = _matrix(dlogits, "dlogits", dev, A * T, V, (logits.dtype,))
 	_enqueue("novic_token_logprobs_bwd", dev, *head, A, T, V, _vector(_given(lse, "lse"), "lse", dev, A * T), *_per_token(grad, "grad", dev, A, T), pd, ldd)

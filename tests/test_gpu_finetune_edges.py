@@ -10,6 +10,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from novic_amd import ops
+from test_gpu_finetune_ops import far_rows, half_step, near
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -117,3 +118,50 @@ def test_policy_of_an_excluded_target():
 		assert not d[0].any() and torch.isfinite(d).all() and bool(d[1, 7] != 0)
 		q = math.exp(6.0) / 300  # the second row's ratio, 1.34: above the range, but the advantage is negative; the first row's is 0 and held at 0.8
 		assert abs(float(stats[0]) - (q + 0.8) * 1.5 / 2) <= 1e-5 and float(stats[2]) == 0.5
+
+
+VOCABULARIES = [5, 130, 500, 900, 1500, 5000, 10007, 20001, 40_001, 70_001]  # every form of the gradient
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V", VOCABULARIES)
+def test_log_probability_gradient_of_far_rows(V, dtype):
+	"""Rows near any level, masked throughout among them: the gradient is that of the row, whose normaliser the fp32 log-sum-exp beside it no longer holds."""
+	A, T = 8, 14
+	x, target, p, lp, bound = far_rows(A * T, V, dtype)
+	target = target.view(A, T)
+	g = torch.Generator(device=DEV).manual_seed(V)
+	out, lse, d, grad = torch.empty(A, T, device=DEV), torch.empty(A * T, device=DEV), torch.empty_like(x), torch.randn(A, T, generator=g, device=DEV)
+	ops.token_logprobs(x, target, out, lse=lse)
+	onehot = torch.zeros_like(p).scatter_(1, target.view(-1, 1), 1.0)
+	ops.token_logprobs_bwd(x, target, lse, grad, d)
+	ref = grad.double().view(-1, 1) * (onehot - p)
+	near(d, ref, grad.double().abs().view(-1, 1) * bound[:, None] * (p + onehot) * 3 + half_step(ref, dtype), f"V = {V}")
+	ops.token_logprobs_bwd(x, target, lse, grad, x)
+	assert torch.equal(x, d)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V", VOCABULARIES)
+def test_log_probability_gradient_of_offset_rows(V, dtype):
+	"""Ordinary logits on levels up to 60 000, where the log-sum-exp's rounding is up to 2^-9 of every probability: the sums' own accuracy, exponents d from the maximum being off by
+	d U and a sum by 96 U.  And a log-sum-exp that is not the row's (of a vocabulary of which these are some columns): the gradient takes it as it is, rounding and all."""
+	A, T = 5, 16
+	g = torch.Generator(device=DEV).manual_seed(V + 1)
+	level = torch.tensor([0.0, 200.0, -200.0, 260.0, -300.0, 4000.0, -4000.0, 60_000.0], device=DEV)[torch.arange(A * T, device=DEV) % 8]
+	x = (2 * torch.randn(A * T, V, generator=g, device=DEV) + level[:, None]).to(dtype)
+	target, grad = torch.randint(0, V, (A, T), generator=g, device=DEV), torch.randn(A, T, generator=g, device=DEV)
+	out, lse, d = torch.empty(A, T, device=DEV), torch.empty(A * T, device=DEV), torch.empty_like(x)
+	ops.token_logprobs(x, target, out, lse=lse)
+	exact = torch.logsumexp(x.double(), 1)
+	onehot = torch.zeros(A * T, V, device=DEV, dtype=torch.double).scatter_(1, target.view(-1, 1), 1.0)
+	dist = (x.double() - x.double().amax(1, keepdim=True)).abs()
+	coef = grad.double().view(-1, 1)
+	other = lse + 8.0
+	for given, norm, taken in ((lse, torch.where(lse.abs() > 256, exact, lse.double()), lse.abs() <= 256), (other, other.double(), torch.ones_like(lse, dtype=torch.bool))):
+		ops.token_logprobs_bwd(x, target, given, grad, d)
+		p = (x.double() - norm[:, None]).exp()
+		ref = coef * (onehot - p)
+		rel = (96 + 12) * U + 2 * U * dist + 3 * U * (given.double().abs() * taken)[:, None]  # (what is taken as given rounds in x - lse)
+		bound = coef.abs() * (p * rel + 3 * U * onehot)
+		near(d, ref, bound + half_step(ref.abs() + bound, dtype), f"V = {V}")
