@@ -295,7 +295,7 @@ struct TeamRow {
 	__device__ __forceinline__ static Point at_max(float m) { return point(LANES == 64 ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(m))) : m); }
 	__device__ __forceinline__ void sum(int V, int lane, float& m, float& s) {
 		m = top();
-		const Point at_m = at_max(m);
+		const Point at_m = at_max(m == -INFINITY ? 0.f : m);  // (nothing but -inf: a sum of zeros, whose logarithm is -inf)
 		here(V, lane);
 		float t = 0.f;
 #pragma unroll

@@ -165,3 +165,16 @@ def test_log_probability_gradient_of_offset_rows(V, dtype):
 		rel = (96 + 12) * U + 2 * U * dist + 3 * U * (given.double().abs() * taken)[:, None]  # (what is taken as given rounds in x - lse)
 		bound = coef.abs() * (p * rel + 3 * U * onehot)
 		near(d, ref, bound + half_step(ref.abs() + bound, dtype), f"V = {V}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("A,V", [(3, 5), (3, 100), (3, 1500), (3, 5000), (4200, 5000), (3, 70_001)])
+def test_log_sum_exp_of_rows_of_nothing(A, V, dtype):
+	"""A row of -inf throughout has no probabilities (NaN) and the log-sum-exp -inf, by every form; its neighbours are untouched."""
+	x = torch.zeros(A, V, device=DEV, dtype=dtype)
+	x[1] = float("-inf")
+	out, lse = torch.empty(A, 1, device=DEV), torch.empty(A, device=DEV)
+	ops.token_logprobs(x, torch.zeros(A, 1, dtype=torch.int64, device=DEV), out, lse=lse)
+	rest = torch.arange(A, device=DEV) != 1
+	assert float(lse[1]) == float("-inf") and bool(out[1].isnan().all())
+	assert bool(((lse[rest] - math.log(V)).abs() <= 8 * U * math.log(V)).all()) and bool(((out[rest] + math.log(V)).abs() <= 8 * U * math.log(V)).all())
