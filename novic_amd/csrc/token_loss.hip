@@ -553,7 +553,8 @@ __device__ __forceinline__ void pref_terms(const Pref& g, int i, double z) {
 	double l;
 	if (g.kind == NOVIC_PREF_SIGMOID) {
 		const double soft = log1p(exp(-fabs(z)));  // -log sigmoid(z) = soft + max(-z, 0)
-		l = (1.0 - g.smoothing) * (soft + fmax(-z, 0.0)) + g.smoothing * (soft + fmax(z, 0.0));
+		l = (1.0 - g.smoothing) * (soft + fmax(-z, 0.0));
+		if (g.smoothing != 0.0) l += g.smoothing * (soft + fmax(z, 0.0));  // (a margin of +inf, whose rejected label has an excluded token, costs nothing without it)
 	} else if (g.kind == NOVIC_PREF_HINGE) {
 		l = z < 1.0 ? 1.0 - z : (z >= 1.0 ? 0.0 : z);
 	} else {

@@ -178,3 +178,22 @@ def test_log_sum_exp_of_rows_of_nothing(A, V, dtype):
 	rest = torch.arange(A, device=DEV) != 1
 	assert float(lse[1]) == float("-inf") and bool(out[1].isnan().all())
 	assert bool(((lse[rest] - math.log(V)).abs() <= 8 * U * math.log(V)).all()) and bool(((out[rest] + math.log(V)).abs() <= 8 * U * math.log(V)).all())
+
+
+@pytest.mark.parametrize("n,V", [(2, 300), (520, 700), (3, 70_001)])
+def test_preference_with_an_excluded_target(n, V):
+	"""A rejected label with a token whose logit is -inf: margin +inf, loss and slope 0 without smoothing, an infinite loss with it; for the preferred label the other way round."""
+	x = torch.zeros(2 * n, V, device=DEV)
+	target, ref = torch.full((2 * n, 1), 3, device=DEV), torch.full((2 * n, 1), -math.log(V), device=DEV)
+	x[n, 3] = float("-inf")  # the first pair's rejected label
+	stats, margin, d = torch.empty(3, device=DEV), torch.empty(n, device=DEV), torch.full_like(x, 7.0)
+	ops.preference_loss(x, target, ref, stats, beta=0.5, margin=margin, dlogits=d)
+	assert float(margin[0]) == float("inf") and bool((margin[1:].abs() <= 64 * U * math.log(V)).all())
+	want = (n - 1) * math.log(2) / n
+	assert abs(float(stats[0]) - want) <= 64 * U * math.log(V) + 8 * U * want and float(stats[1]) == float("inf")
+	assert not d[0].any() and not d[n].any() and torch.isfinite(d).all() and bool((d[1:n, 3] < 0).all())
+	ops.preference_loss(x, target, ref, stats, beta=0.5, smoothing=0.1)
+	assert float(stats[0]) == float("inf")
+	x[n, 3], x[0, 3] = 0.0, float("-inf")
+	ops.preference_loss(x, target, ref, stats, beta=0.5, margin=margin)
+	assert float(margin[0]) == -float("inf") and float(stats[0]) == float("inf")
