@@ -535,19 +535,24 @@ struct Pref {
 };
 __device__ __forceinline__ double pref_margin(const Pref& g, double up, double un) { return g.beta * (up - un); }
 __device__ __forceinline__ float pref_weight(const Pref& g, int i) { return g.weight ? g.weight[i] : 1.f; }
-// gradient of sum_i w_i l_i to u of pair i's preferred sequence (the other's is its negative): a sigmoid's small side is formed by itself, without a difference
+// gradient of sum_i w_i l_i to u of pair i's preferred sequence (the other's is its negative).  A sigmoid's small side is formed by itself, without a difference, in fp32; the square
+// form and the products are fp64: 1 / beta^2 may leave fp32 where the slope, which takes beta once more, does not.
 __device__ __forceinline__ float pref_slope(const Pref& g, int i, double z) {
-	float dz;
-	if (g.kind == NOVIC_PREF_SIGMOID) {
-		const float e = expf(-fabsf((float)z)), small = e / (1.f + e), large = 1.f / (1.f + e);
-		const float at = z < 0.0 ? small : large, rest = z < 0.0 ? large : small;  // sigmoid(z), sigmoid(-z)
-		dz = (float)g.smoothing * at - (1.f - (float)g.smoothing) * rest;
-	} else if (g.kind == NOVIC_PREF_HINGE) {
-		dz = z < 1.0 ? -1.f : (z >= 1.0 ? 0.f : (float)z);  // (a NaN stays one)
+	double du;
+	if (g.kind == NOVIC_PREF_SQUARE) {
+		du = 2.0 * (z - 0.5) / g.beta;
 	} else {
-		dz = (float)(2.0 * (z - 0.5) / (g.beta * g.beta));
+		float dz;
+		if (g.kind == NOVIC_PREF_SIGMOID) {
+			const float e = expf(-fabsf((float)z)), small = e / (1.f + e), large = 1.f / (1.f + e);
+			const float at = z < 0.0 ? small : large, rest = z < 0.0 ? large : small;  // sigmoid(z), sigmoid(-z)
+			dz = (float)g.smoothing * at - (1.f - (float)g.smoothing) * rest;
+		} else {
+			dz = z < 1.0 ? -1.f : (z >= 1.0 ? 0.f : (float)z);  // (a NaN stays one)
+		}
+		du = (double)dz * g.beta;
 	}
-	return pref_weight(g, i) * dz * (float)g.beta;
+	return (float)((double)pref_weight(g, i) * du);
 }
 __device__ __forceinline__ void pref_terms(const Pref& g, int i, double z) {
 	double l;

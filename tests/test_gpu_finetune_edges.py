@@ -197,3 +197,18 @@ def test_preference_with_an_excluded_target(n, V):
 	x[n, 3], x[0, 3] = 0.0, float("-inf")
 	ops.preference_loss(x, target, ref, stats, beta=0.5, margin=margin)
 	assert float(margin[0]) == -float("inf") and float(stats[0]) == float("inf")
+
+
+@pytest.mark.parametrize("n,V", [(2, 300), (520, 700), (3, 70_001)])
+def test_preference_of_a_small_beta(n, V):
+	"""The square form at beta = 3e-20: loss (1 / (2 beta))^2 = 2.8e38, slope 1 / beta = 3.3e19, both fp32 numbers; their way there (1 / beta^2 = 1.1e39) is not."""
+	beta = 3e-20
+	x, target, ref = torch.zeros(2 * n, V, device=DEV), torch.full((2 * n, 1), 3, device=DEV), torch.full((2 * n, 1), -math.log(V), device=DEV)
+	stats, d = torch.empty(3, device=DEV), torch.empty_like(x)
+	ops.preference_loss(x, target, ref, stats, beta=beta, kind="square", dlogits=d)
+	assert abs(float(stats[0]) - 0.25 / beta ** 2) <= 8 * U * 0.25 / beta ** 2  # (u, some 1e-6, adds nothing to 1 / (2 beta))
+	want = torch.full((2 * n, V), 1.0 / V, device=DEV, dtype=torch.double)
+	want[:, 3] -= 1
+	want[n:] *= -1
+	want *= 1 / beta / n
+	near(d, want, (96 + 16) * U * want.abs())
