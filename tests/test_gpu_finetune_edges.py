@@ -10,6 +10,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from novic_amd import ops
+import test_gpu_finetune_ops as whole  # (its tests at other sizes; imported by name they would be collected here once more)
 from test_gpu_finetune_ops import far_rows, half_step, near
 
 pytestmark = pytest.mark.gpu
@@ -212,3 +213,36 @@ def test_preference_of_a_small_beta(n, V):
 	want[n:] *= -1
 	want *= 1 / beta / n
 	near(d, want, (96 + 16) * U * want.abs())
+
+
+@pytest.mark.parametrize("per_seq", [False, True])
+@pytest.mark.parametrize("A,T,V,dtype", [(1300, 7, 97, BF16), (20_000, 5, 33, F32), (20_000, 5, 33, F16), (90, 300, 40, F32), (2500, 40, 65, BF16), (700, 12, 3000, BF16)])
+def test_policy_of_many_rows(A, T, V, dtype, per_seq):
+	"""Row counts at which the counts come from a launch of their own (several lanes a sequence, several sequences a lane) and the four means from slices."""
+	whole.test_policy(A, T, V, 3, 1, dtype, 0.1, 2, per_seq)
+	whole.test_policy(A, T, V, 0, 0, dtype, 0.0, 1, per_seq)
+
+
+@pytest.mark.parametrize("dtype,n,T,V", [(BF16, 4097, 2, 600), (F32, 4099, 3, 300), (F16, 8191, 1, 2500), (BF16, 4097, 9, 700), (F32, 5001, 2, 40)])
+def test_preference_of_many_weighted_pairs(dtype, n, T, V):
+	"""More pairs than whose weights every workgroup adds up for itself (odd counts: with weights, the first of them 0)."""
+	whole.test_preference(n, T, V, 3, 1, dtype, "sigmoid", 0.1, 0.3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("E", [5, 97, 509, 1280, 5001, 9000, 16384])
+def test_layernorm_backward_over_its_inputs(E, dtype):
+	"""dx written over x, and over dy, with and without the residual's gradient: the bits of the one written beside them; both affine gradients too."""
+	g = torch.Generator(device=DEV).manual_seed(E)
+	rows = 700
+	rnd = lambda: torch.randn(rows, E, generator=g, device=DEV).to(dtype)  # noqa: E731
+	x, dy, resid, gamma = rnd(), rnd(), rnd(), torch.randn(E, generator=g, device=DEV)
+	mean, rstd = x.float().mean(1), (x.float().var(1, unbiased=False) + 1e-5).rsqrt()
+	for dx_in in (None, resid):
+		dx, dgamma, dbeta = torch.empty_like(x), torch.empty(E, device=DEV), torch.empty(E, device=DEV)
+		ops.layernorm_stats_bwd(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, dx_in=dx_in)
+		for over in ("x", "dy"):
+			a, b, dg, db = x.clone(), dy.clone(), torch.empty(E, device=DEV), torch.empty(E, device=DEV)
+			out = a if over == "x" else b
+			ops.layernorm_stats_bwd(b, a, gamma, mean, rstd, out, dg, db, dx_in=dx_in)
+			assert torch.equal(out, dx) and torch.equal(dg, dgamma) and torch.equal(db, dbeta), over
