@@ -61,11 +61,11 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, fwd_waves(LANES, NC * CH
 	RawVec<XT, CH> raw[NC], next[NC];
 	const int first = blockIdx.x * TEAMS + team;
 	if (first < rows) load(raw, first);
-	// (teams of more than a wave have a block of their own, so the rows of a block and with them the barriers in team_sum2 are the same for all its threads.  Unsigned: the row
-	// behind the last, up to a stride of 16384 beyond 2^31, is no int)
-	for (unsigned row0 = first; row0 < (unsigned)rows; row0 += stride) {
-		const int row = LANES < 64 ? row0 : __builtin_amdgcn_readfirstlane(row0);
-		load(next, min(row0 + stride, (unsigned)rows - 1));  // requested before this row is reduced
+	// (teams of more than a wave have a block of their own, so the rows of a block and with them the barriers in team_sum2 are the same for all its threads.  What is left is counted
+	// down: the row behind the last, up to a stride of 16384 beyond 2^31, is no int)
+	for (int left = rows - first; left > 0; left -= stride) {
+		const int row0 = rows - left, row = LANES < 64 ? row0 : __builtin_amdgcn_readfirstlane(row0);
+		load(next, rows - max(left - stride, 1));  // requested before this row is reduced
 		float s = 0.f, q = 0.f, off = 0.f, none = 0.f;
 #pragma unroll
 		for (int c = 0; c < NC; ++c) {
@@ -158,13 +158,14 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_stats_bwd
 		r.rs = rstd[row];
 	};
 	const int stride = gridDim.x * TEAMS;
-	unsigned row = blockIdx.x * TEAMS + team;  // (unsigned as in the forward kernel)
+	int row = blockIdx.x * TEAMS + team;
 	if (LANES >= 64) row = __builtin_amdgcn_readfirstlane(row);
 	Row cur;
-	if (AHEAD && row < (unsigned)rows) load(cur, row);
-	for (; row < (unsigned)rows; row += stride) {
+	if (AHEAD && row < rows) load(cur, row);
+	for (int left = rows - row; left > 0; left -= stride) {  // (counted down as in the forward kernel)
+		row = rows - left;
 		Row nxt;
-		if (AHEAD) load(nxt, min(row + stride, (unsigned)rows - 1));
+		if (AHEAD) load(nxt, rows - max(left - stride, 1));
 		else load(cur, row);
 		float s1 = 0.f, s2 = 0.f;
 #pragma unroll
