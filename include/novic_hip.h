@@ -542,8 +542,8 @@ int novic_token_logprobs_bwd(const void* logits, int type, int64_t ldl, const vo
                              const float* lse, const float* grad, int64_t grad_lda, int64_t grad_ldt, void* dlogits, int64_t ldd, hipStream_t stream);
 
 /* Preference loss of n pairs: sequence i of the 2 n is preferred to sequence n + i.  z_i = beta (sum_t (logp - ref) of i - the same of n + i) over counted rows;
- * loss = sum_i w_i l(z_i) / sum_i w_i (weight NULL: ones; no weight at all: loss and gradient are 0), l = -(1 - smoothing) log sigmoid(z) - smoothing log sigmoid(-z) |
- * max(0, 1 - z) | ((z - 1/2) / beta)^2.  stats [3] = loss, weighted mean of z, sum of the weights; margin [n] = z, logp, dlogits = grad_scale dloss/dlogits may each be NULL. */
+ * loss = sum_i w_i l(z_i) / sum_i w_i (weight NULL: ones; no weight at all: loss and gradient are 0), l = -(1 - smoothing) log sigmoid(z) - smoothing log sigmoid(-z) (smoothing
+ * 0: no second term, whatever z) | max(0, 1 - z) | ((z - 1/2) / beta)^2.  n <= 2^29.  stats [3] = loss, weighted mean of z, sum of the weights; margin [n] = z, logp, dlogits = grad_scale dloss/dlogits may each be NULL. */
 enum { NOVIC_PREF_SIGMOID = 0, NOVIC_PREF_HINGE = 1, NOVIC_PREF_SQUARE = 2 };
 uint64_t novic_preference_loss_ws(int n, int T);
 int novic_preference_loss(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int n, int T, int V,
@@ -552,6 +552,7 @@ int novic_preference_loss(const void* logits, int type, int64_t ldl, const void*
 
 /* Clipped policy loss: q = exp(logp - old), a = adv[a adv_lda + t adv_ldt]: -min(q a, clip(q, 1 - clip_lo, 1 + clip_hi) a) + kl_coef (exp(ref - logp) - (ref - logp) - 1) (ref NULL:
  * no such term), averaged over the counted rows, or (per_sequence) over the sequences that have any of the average over each one's counted rows; no counted row: all zeros.
+ * An advantage of 0 and a kl_coef of 0 leave their terms out, also where the exponential beside them is beyond any number (the KL is still reported).
  * stats [4] = loss, KL, share of clipped rows (averaged the same way), counted rows; logp, dlogits = grad_scale dloss/dlogits may be NULL. */
 uint64_t novic_policy_loss_ws(int A, int T);
 int novic_policy_loss(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int A, int T, int V,

@@ -8,9 +8,12 @@
 //                    the mean over a sequence's counted rows
 //
 // HBM-bound: V logits a row in, V gradients a row out.  A row belongs to a workgroup that holds it in registers between the sum and the gradient; padded rows are not read.
-// The exponentials and the sums over the vocabulary are fp32; a log-probability is formed and added up over its sequence in fp64 (a handful of operations a ROW):
-// the losses take differences of sums that nearly cancel.  MI355X: gradient of log-probabilities over [4928 x 49408] fp16 134 us (733 MB, 5.5 TB/s); preference step of 4096 pairs of
-// [7 x 6912] bf16 250 us (1249 MB, 5.0 TB/s), policy step of as many rows 218 us (5.7 TB/s).
+// Exponentials, sums over the vocabulary and the logarithm of such a sum are fp32; what they give is added to the maximum, and up over a sequence, in fp64 (a handful of operations
+// a ROW): the losses take differences of sums that nearly cancel.  A log-probability is off by some 1e-7: at 7 000 to 50 000 columns of scale 2 by -5e-8 on average (log2 e rounds
+// down, which makes the exponentials below the maximum a little large), 5e-8 to 7e-8 rms about that.  The average adds up over a sequence, to 1.7e-5 in 333 tokens, where the rounding
+// of their fp32 reference values (up to 2^-21 each at -10) adds 5e-6.  A second part of log2 e does not mend it: most of it is lost in the rounding of the fp32 exponent.
+// MI355X: gradient of log-probabilities over [4928 x 49408] fp16 137 us (733 MB, 5.4 TB/s); preference step of 4096 pairs of [7 x 6912] bf16 250 us (1249 MB, 5.0 TB/s), policy step
+// of as many rows 219 us (5.7 TB/s); each back to back, some 20 us more for a call that finds the GPU idle.
 #include "novic_hip.h"
 #include "rowvec.hpp"
 
@@ -62,7 +65,7 @@ __device__ __forceinline__ int row_index(const Rows& g) {
 	return r < (long long)g.A * g.T ? (int)r : -1;
 }
 
-// log(s) to 1e-16 relative of a sum (up to 2^64 V) without the cost of a double-precision logarithm: s = 2^k f, f in [0.7, 1.42): |logf(f)| < 0.36, its rounding 3e-8 absolute
+// log(s) of a sum to 3e-8 ABSOLUTE, however large, without the cost of a double-precision logarithm: s = 2^k f, f in [0.7, 1.42), |logf(f)| < 0.36; the sum itself is off by more
 __device__ __forceinline__ double log_wide(float s) {
 	int k;
 	float f = frexpf(s, &k);
@@ -690,8 +693,8 @@ __global__ __launch_bounds__(1024) void pref_finish_kernel(const Pref g) {
 // A pair by one workgroup, loss and gradient.  The pair's rows (at most 64) are lanes' business first: each wave asks for all targets and reference values and knows the rows that
 // count from a ballot.  Those are dealt to the waves in turn; the row that a wave sums last stays in its registers up to its gradient, any others are read again (a pair's
 // time later: out of L2 or the memory-side cache).  Sixteen vectors a lane are what 128 registers hold beside the rest of the kernel.  Bound by the rows in flight: between a pair's
-// reading and its writing stands a barrier, and two workgroups a unit are what covers it.  4096 pairs of 7 + 7 rows of 6912 bf16: 249 us with eight waves, with four 272, with five 261,
-// with six 254.  Second rows kept in LDS instead of read again: 1 % less.
+// reading and its writing stands a barrier, and two workgroups a unit are what covers it.  4096 pairs of 7 + 7 rows of 6912 bf16: 249 us with eight waves, with four 272.
+// Second rows kept in LDS instead of read again: 1 % less.
 constexpr int PAIR_ROWS = 64, PAIR_VECTORS = 16, PAIR_WEIGHTS = 4096;
 template <typename T, int CH, int NC, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void pref_pair_kernel(const Rows g, const LogpOut o, const Pref q) {
@@ -1218,7 +1221,7 @@ extern "C" uint64_t novic_preference_loss_ws(int n, int T) {
 extern "C" int novic_preference_loss(const void* logits, int type, int64_t ldl, const void* target, int tok_bytes, int64_t ldt, const uint8_t* pad, int64_t ldp, int n, int T, int V,
                                      const float* ref, int64_t ldref, const float* weight, int kind, double beta, double smoothing, double grad_scale, float* logp, int64_t ldo,
                                      float* margin, void* dlogits, int64_t ldd, float* stats, void* ws, uint64_t ws_bytes, hipStream_t stream) {
-	NOVIC_CHECK(n >= 1 && n <= (1 << 29) && T >= 1, "novic_preference_loss: at least one pair and one position");
+	NOVIC_CHECK(n >= 1 && n <= (1 << 29) && T >= 1, "novic_preference_loss: at least one pair and one position, at most 2^29 pairs");
 	Rows g = {logits, ldl, dlogits, ldd, target, pad, ldt, ldp, tok_bytes, 2 * n, T, V};
 	const char* bad = rows_bad(g, type);
 	NOVIC_CHECK(!bad, bad);
